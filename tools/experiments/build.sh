@@ -9,7 +9,7 @@ set -e
 cd "$(dirname "$0")"
 LIB=../../bmt_amd/lib
 [ -f "$LIB/obj/runtime.o" ] || bash ../../bmt_amd/csrc/build.sh
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wno-unused-result -I../../bmt_amd/csrc"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops -I../../bmt_amd/csrc"
 if [ ! -f exp_lib.o ] || [ exp_lib.hip -nt exp_lib.o ] || [ attn_fwd32.hip -nt exp_lib.o ] || [ ../../bmt_amd/csrc/attention_bf16.hip -nt exp_lib.o ]; then
   hipcc $FLAGS $BMT_EXP_FLAGS -c exp_lib.hip -o exp_lib.o
 fi
