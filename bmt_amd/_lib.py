@@ -194,6 +194,19 @@ SIGNATURES = {
     "bmt_loss_finish": (i32, [vp, vp, vp, vp, vp]),
     "bmt_layernorm_bwd_partial2": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, i64, vp, i32, i32, vp, vp]),
     "bmt_layernorm_bwd_emit": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, i64, vp, vp, i64, f32, vp, u32, i32, i32, vp, vp]),
+    "bmt_logp_rows": (i32, [vp, i32, i64, i64, i32, i32, i32, vp, i64, i64, vp, i64, i64, i64, vp, vp, vp]),
+    "bmt_logit_grad": (i32, [vp, i32, i64, i64, i32, i32, i32, vp, i64, i64, vp, i64, i64, i64, vp, vp, i64, i64, vp, i32, vp, i64, i64, vp]),
+    "bmt_policy_ws_bytes": (i64, [i32, i32]),
+    "bmt_policy_loss": (i32, [vp, i32, i64, i64, i32, i32, i32, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, f32, f32, f32, i32, vp, vp, vp,
+                              vp, i64, vp, i64, i64, vp]),
+    "bmt_preference_ws_bytes": (i64, [i32, i32]),
+    "bmt_preference_loss": (i32, [vp, i32, i64, i64, i32, i32, i32, vp, i64, i64, vp, i64, i64, i64, vp, i64, f32, f32, i32, vp, vp, vp, i64, vp]),
+    "bmt_embedding": (i32, [vp, vp, i64, vp, i64, i32, i32, i32, f32, vp]),
+    "bmt_embedding_bwd_ws_bytes": (i64, [i64, i32, i32]),
+    "bmt_embedding_bwd": (i32, [vp, vp, i64, i64, i32, i32, i32, f32, i64, vp, vp, i64, vp, i64, vp]),
+    "bmt_clip_tile_bytes": (i32, []),
+    "bmt_clip_ws_bytes": (i64, []),
+    "bmt_clip_grads": (i32, [vp, i32, i32, f32, f32, vp, i32, i32, vp, vp, i64, vp]),
     "bmt_adam_step": (i32, [vp, vp, i32, i64, vp, f32, f32, f32, f32, f32, vp, vp]),
     "bmt_grad_sqnorm": (i32, [vp, vp, i32, i64, vp, f32, vp, vp]),
     "bmt_scale_tensors": (i32, [vp, vp, i32, i64, vp, vp]),

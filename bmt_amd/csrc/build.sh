@@ -14,7 +14,7 @@ FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wno-unused-resul
 # objects are kept per flag set; `build.sh all` compiles every source again
 ALL=${1:-}
 [ "$(cat "$OUT/$OBJ/flags" 2>/dev/null)" = "$FLAGS" ] || ALL=all
-SRCS="runtime gemm_bf16 attention attention_bf16 norm elementwise loss optim proposal postprocess ingest raw_memory rank_attn"
+SRCS="runtime gemm_bf16 attention attention_bf16 norm elementwise loss optim proposal postprocess ingest raw_memory rank_attn tuning_loss embedding grad_clip"
 pids=()
 for f in $SRCS; do
   if [ "$ALL" = all ] || [ ! -f "$OUT/$OBJ/$f.o" ] || [ "$f.hip" -nt "$OUT/$OBJ/$f.o" ] || [ common.h -nt "$OUT/$OBJ/$f.o" ] || [ ../../include/bmt_hip.h -nt "$OUT/$OBJ/$f.o" ]; then

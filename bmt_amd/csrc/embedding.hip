@@ -1,0 +1,420 @@
+// Scaled embedding lookup and its gradient by sorted tokens.
+//   out[n] = scale W[id_n]                              dW[v] = scale sum_{n : id_n = v} dout[n]
+// Bound: HBM -- the lookup reads N rows and writes N rows, the gradient reads N rows and writes V rows, one or two operations per element.
+// The gradient sums in fp32 over the positions of a token in ascending order, rounded once: no atomics, the same bits on every run.  Three launches:
+//   order  every workgroup owns a range of the vocabulary, reads ALL ids (they come from L2: 8 bytes against a row of hundreds) and places the
+//          positions of its tokens, in order, behind the count of the tokens below its range -- no second pass over a global histogram
+//   sum    a wave per (token, block of columns) adds a token's rows if they are at most EMB_LONG; the rows of more frequent tokens are added
+//          EMB_LONG sorted positions at a time by workgroups of their own (a few tokens hold half of a text)
+//   join   adds those partial sums per token, in order
+#include "common.h"
+
+namespace {
+
+constexpr int EMB_LONG = 32;        // positions a wave adds by itself; also the sorted positions per partial sum: a longer run starts in at most one of them
+constexpr int EMB_BINS = 960;       // most tokens a workgroup of the order kernel owns: one per thread in its scan, 60 KB of LDS
+
+__device__ __forceinline__ int clamp_id(int64_t id, int V) { return id < 0 ? 0 : (id >= V ? V - 1 : (int)id); }
+
+template <int BYTES>
+struct Vec;
+template <>
+struct Vec<16> { typedef u32x4 T; };
+template <>
+struct Vec<8> { typedef u32x2 T; };
+template <>
+struct Vec<4> { typedef uint32_t T; };
+template <>
+struct Vec<2> { typedef uint16_t T; };
+
+template <int DT>
+constexpr int elem_size() { return DT == BMT_DT_F32 ? 4 : 2; }
+// G elements (16, 8 or one element's bytes) at p <-> floats
+template <int DT, int G>
+struct Cols {
+    typedef typename Vec<elem_size<DT>() * G>::T T;
+    static __device__ __forceinline__ T load(const char* p) { return *reinterpret_cast<const T*>(p); }
+    static __device__ __forceinline__ uint32_t word(const T& v, int i) {
+        if constexpr (sizeof(T) <= 4) return (uint32_t)v;
+        else return v[i];
+    }
+    static __device__ __forceinline__ void get(const T& v, float (&x)[G]) {
+        if constexpr (DT == BMT_DT_F32) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) x[j] = __uint_as_float(word(v, j));
+        } else {
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                const uint32_t h = (word(v, j / 2) >> ((j & 1) * 16)) & 0xffffu;
+                x[j] = DT == BMT_DT_BF16 ? bf_bits2f(h) : h_bits2f(h);
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(char* p, const float (&x)[G]) {
+        T v;
+        if constexpr (DT == BMT_DT_F32) {
+            if constexpr (G == 1) v = __float_as_uint(x[0]);
+            else {
+#pragma unroll
+                for (int j = 0; j < G; ++j) v[j] = __float_as_uint(x[j]);
+            }
+        } else if constexpr (G == 1) {
+            v = (uint16_t)(pack_2<DT == BMT_DT_F16>(x[0], 0.f) & 0xffffu);
+        } else {
+#pragma unroll
+            for (int j = 0; j < G / 2; ++j) v[j] = pack_2<DT == BMT_DT_F16>(x[2 * j], x[2 * j + 1]);
+        }
+        *reinterpret_cast<T*>(p) = v;
+    }
+};
+
+// ---------------------------------------------------------------- lookup: a wave per (TPW tokens, block of 64 G columns)
+template <int DT, int G, int TPW>
+__global__ __launch_bounds__(256) void embed_kernel(const int64_t* __restrict__ ids, const char* __restrict__ W, int64_t ldw, char* __restrict__ out, int64_t N, int D,
+                                                     int V, float scale, int ncb, int64_t tasks) {
+    constexpr int E = elem_size<DT>();
+    const int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (task >= tasks) return;
+    const int64_t n0 = task / ncb * TPW;
+    const int c = ((int)(task % ncb) * 64 + (threadIdx.x & 63)) * G;
+    if (c >= D) return;
+    typename Cols<DT, G>::T v[TPW];
+#pragma unroll
+    for (int i = 0; i < TPW; ++i)
+        if (n0 + i < N) v[i] = Cols<DT, G>::load(W + ((int64_t)clamp_id(ids[n0 + i], V) * ldw + c) * E);
+#pragma unroll
+    for (int i = 0; i < TPW; ++i)
+        if (n0 + i < N) {
+            float x[G];
+            Cols<DT, G>::get(v[i], x);
+#pragma unroll
+            for (int j = 0; j < G; ++j) x[j] *= scale;
+            Cols<DT, G>::store(out + ((n0 + i) * D + c) * E, x);
+        }
+}
+
+// ---------------------------------------------------------------- order: stable counting sort, a range of tokens per workgroup
+// Wave w walks the ids [w * chunk, (w + 1) * chunk); K > 0: a lane keeps its K ids in registers between counting and placing (N <= 1024 K),
+// K = 0: they are read twice.  offsets[v] = first sorted position of token v, offsets[V] = the positions that count (the padding id does not).
+template <int K>
+__global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __restrict__ ids, int64_t N, int V, int64_t pad, int nb, int* __restrict__ offsets,
+                                                            int* __restrict__ order, int* __restrict__ token) {
+    extern __shared__ int hist[];      // [16][nb]
+    __shared__ int wsum[16], wbelow[16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int v0 = blockIdx.x * nb, nv = min(nb, V - v0);
+    for (int i = threadIdx.x; i < 16 * nb; i += 1024) hist[i] = 0;
+    __syncthreads();
+    const int64_t chunk = ((N + 15) / 16 + 63) / 64 * 64, first = wave * chunk, last = min(N, first + chunk);
+    int* mine = hist + wave * nb;
+    int key[K > 0 ? K : 1];      // the token relative to the range; below it: negative; the padding id and positions behind the end: INT_MAX
+    int below = 0;
+    auto fetch = [&](int64_t n) -> int {
+        if (n >= last) return 0x7fffffff;
+        const int64_t id = ids[n];
+        return id == pad ? 0x7fffffff : clamp_id(id, V) - v0;
+    };
+    auto count = [&](int k) {
+        if (k < 0) ++below;
+        else if (k < nv) atomicAdd(&mine[k], 1);
+    };
+    if constexpr (K > 0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) key[i] = fetch(first + i * 64 + lane);
+#pragma unroll
+        for (int i = 0; i < K; ++i) count(key[i]);
+    } else {
+        for (int64_t n = first; n < last; n += 64 * 8) {
+            int k8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) k8[i] = fetch(n + i * 64 + lane);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) count(k8[i]);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, 64);
+    if (lane == 0) wbelow[wave] = below;
+    __syncthreads();
+    // exclusive scan of the tokens' totals (one token per thread), then of each token's counts over the waves
+    int total = 0;
+    if ((int)threadIdx.x < nv)
+        for (int w = 0; w < 16; ++w) total += hist[w * nb + threadIdx.x];
+    int scan = total;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(scan, o, 64);
+        if (lane >= o) scan += up;
+    }
+    if (lane == 63) wsum[wave] = scan;
+    __syncthreads();
+    int start = scan - total;
+    for (int w = 0; w < 16; ++w) {
+        start += wbelow[w];
+        if (w < wave) start += wsum[w];
+    }
+    if ((int)threadIdx.x < nv) {
+        offsets[v0 + threadIdx.x] = start;
+        if (v0 + (int)threadIdx.x == V - 1) offsets[V] = start + total;
+        for (int w = 0, at = start; w < 16; ++w) {
+            const int h = hist[w * nb + threadIdx.x];
+            hist[w * nb + threadIdx.x] = at;
+            at += h;
+        }
+    }
+    __syncthreads();
+    auto place = [&](int k, int64_t n) {      // 64 positions: the lanes of one token at a time, in lane order
+        const bool in = k >= 0 && k < nv;
+        uint64_t todo = __ballot(in);
+        while (todo) {
+            const int lead = __ffsll((unsigned long long)todo) - 1, kl = __shfl(k, lead, 64);
+            const uint64_t same = __ballot(in && k == kl);
+            int at = 0;
+            if (lane == lead) at = atomicAdd(&mine[kl], (int)__popcll(same));
+            at = __shfl(at, lead, 64);
+            if (in && k == kl) {
+                const int p = at + (int)__popcll(same & ((1ull << lane) - 1));
+                order[p] = (int)n;
+                token[p] = v0 + k;
+            }
+            todo &= ~same;
+        }
+    };
+    if constexpr (K > 0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) place(key[i], first + i * 64 + lane);
+    } else {
+        for (int64_t n = first; n < last; n += 64) place(fetch(n + lane), n + lane);
+    }
+}
+
+// rows order[p0 .. p1) of dout, columns c .. c + G, added in order; a lane outside the columns adds nothing
+template <int DT, int G>
+__device__ __forceinline__ void add_rows(const char* dout, int64_t ld, const int* __restrict__ order, int p0, int p1, int c, bool in, float (&acc)[G]) {
+    constexpr int E = elem_size<DT>(), U = 8;
+    const int lane = threadIdx.x & 63;
+    for (int p = p0; p < p1; p += 64) {
+        const int have = min(64, p1 - p);
+        const int pos = lane < have ? order[p + lane] : 0;
+        for (int i = 0; i < have; i += U) {
+            typename Cols<DT, G>::T v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int n = __builtin_amdgcn_readlane(pos, min(i + u, have - 1));
+                if (in && i + u < have) v[u] = Cols<DT, G>::load(dout + ((int64_t)n * ld + c) * E);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (in && i + u < have) {
+                    float x[G];
+                    Cols<DT, G>::get(v[u], x);
+#pragma unroll
+                    for (int j = 0; j < G; ++j) acc[j] += x[j];
+                }
+        }
+    }
+}
+
+// dW[v] = scale acc, or (into != NULL: a static fp32 gradient buffer) into[v] += scale acc
+template <int DT, int G>
+__device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, int v, int c, float scale, const float (&acc)[G]) {
+    float x[G];
+    if (into) {
+        float* p = into + (int64_t)v * ldw + c;
+#pragma unroll
+        for (int j = 0; j < G; ++j) p[j] += scale * acc[j];
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < G; ++j) x[j] = scale * acc[j];
+    Cols<DT, G>::store(dW + ((int64_t)v * ldw + c) * elem_size<DT>(), x);
+}
+
+// workgroups [0, chunks * ncb): partial sums of the frequent tokens; behind them: a wave per (token, block of columns)
+template <int DT, int G>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__ dout, int64_t ld, const int* __restrict__ offsets, const int* __restrict__ order,
+                                                         const int* __restrict__ token, float* __restrict__ part, int64_t ldp, char* __restrict__ dW,
+                                                         float* __restrict__ into, int64_t ldw, int D, int V, float scale, int chunks, int ncb) {
+    __shared__ float red[3][64 * G];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t wg = blockIdx.x, nlong = (int64_t)chunks * ncb;
+    if (wg < nlong) {
+        const int k = (int)(wg / ncb), c = ((int)(wg % ncb) * 64 + lane) * G;
+        const bool in = c < D;
+        const int p0 = k * EMB_LONG, p1 = min(p0 + EMB_LONG, offsets[V]);
+        if (p0 >= p1) return;
+        const int t0 = token[p0], t1 = token[p1 - 1];
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {      // at most the run that reaches into the chunk and the run that reaches out of it are long
+            const int v = h ? t1 : t0;
+            if (h && t1 == t0) break;
+            const int a = offsets[v], b = offsets[v + 1];
+            if (b - a <= EMB_LONG) continue;
+            const int q0 = max(p0, a), q1 = min(p1, b), each = (q1 - q0 + 3) / 4;
+            float acc[G] = {};
+            add_rows<DT, G>(dout, ld, order, min(q1, q0 + wave * each), min(q1, q0 + (wave + 1) * each), c, in, acc);
+            __syncthreads();
+            if (wave > 0)
+#pragma unroll
+                for (int j = 0; j < G; ++j) red[wave - 1][j * 64 + lane] = acc[j];
+            __syncthreads();
+            if (wave == 0 && in) {
+                float* o = part + (int64_t)(2 * k + h) * ldp + c;
+#pragma unroll
+                for (int j = 0; j < G; ++j) o[j] = ((acc[j] + red[0][j * 64 + lane]) + red[1][j * 64 + lane]) + red[2][j * 64 + lane];
+            }
+        }
+        return;
+    }
+    const int64_t task = (wg - nlong) * 4 + wave;
+    if (task >= (int64_t)V * ncb) return;
+    const int v = (int)(task / ncb), c = ((int)(task % ncb) * 64 + lane) * G;
+    const bool in = c < D;
+    const int a = offsets[v], b = offsets[v + 1];
+    if (b - a > EMB_LONG || (into && a == b)) return;
+    float acc[G] = {};
+    add_rows<DT, G>(dout, ld, order, a, b, c, in, acc);
+    if (in) finish_row<DT, G>(dW, into, ldw, v, c, scale, acc);
+}
+
+// a workgroup per (chunk, block of columns): the frequent token whose run starts in the chunk, if there is one -- it holds the chunk's last position
+template <int DT, int G>
+__global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__ offsets, const int* __restrict__ token, const float* __restrict__ part, int64_t ldp,
+                                                          char* __restrict__ dW, float* __restrict__ into, int64_t ldw, int D, int V, float scale, int ncb) {
+    __shared__ float red[3][64 * G];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int k = blockIdx.x / ncb, c = ((int)(blockIdx.x % ncb) * 64 + lane) * G;
+    const bool in = c < D;
+    const int p0 = k * EMB_LONG, p1 = min(p0 + EMB_LONG, offsets[V]);
+    if (p0 >= p1) return;
+    const int v = token[p1 - 1], a = offsets[v], b = offsets[v + 1];
+    if (a < p0 || b - a <= EMB_LONG) return;
+    const int k1 = (b - 1) / EMB_LONG, n = k1 - k + 1, each = (n + 3) / 4;      // partial sums: slot 0 or 1 of chunk k, slot 0 of the following ones
+    const int i0 = min(n, wave * each), i1 = min(n, (wave + 1) * each);
+    float acc[G] = {};
+    if (in) {
+#pragma unroll 4
+        for (int i = i0; i < i1; ++i) {
+            const float* o = part + (int64_t)(2 * (k + i) + (i == 0 && a > p0 ? 1 : 0)) * ldp + c;
+#pragma unroll
+            for (int j = 0; j < G; ++j) acc[j] += o[j];
+        }
+    }
+    if (wave > 0)
+#pragma unroll
+        for (int j = 0; j < G; ++j) red[wave - 1][j * 64 + lane] = acc[j];
+    __syncthreads();
+    if (wave == 0 && in) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) acc[j] = ((acc[j] + red[0][j * 64 + lane]) + red[1][j * 64 + lane]) + red[2][j * 64 + lane];
+        finish_row<DT, G>(dW, into, ldw, v, c, scale, acc);
+    }
+}
+
+inline int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+inline int64_t emb_ld(int D) { return (D + 7) / 8 * 8; }      // floats per partial sum: 16-byte rows for every G
+
+// elements per lane: 16 or 8 bytes where every row of both sides is aligned to them, else one element
+inline int cols_of(int esize, int D, const void* a, int64_t lda, const void* b, int64_t ldb) {
+    for (int bytes = 16; bytes >= 8; bytes /= 2) {
+        const int64_t g = bytes / esize;
+        if (D % g == 0 && lda % g == 0 && ldb % g == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & (bytes - 1)) == 0) return (int)g;
+    }
+    return 1;
+}
+
+// one workgroup per CU: each reads every id once, so more of them only multiply the reads
+inline int bins_for(int V) {
+    const int nb = bmt_cdiv(V, 256);
+    return nb < EMB_BINS ? nb : EMB_BINS;
+}
+
+#define BMT_EMB_BY(dtype, g, CALL)                                                           \
+    do {                                                                                     \
+        if (dtype == BMT_DT_F32) {                                                           \
+            if (g == 4) CALL(BMT_DT_F32, 4);                                                 \
+            else if (g == 2) CALL(BMT_DT_F32, 2);                                            \
+            else CALL(BMT_DT_F32, 1);                                                        \
+        } else if (dtype == BMT_DT_BF16) {                                                   \
+            if (g == 8) CALL(BMT_DT_BF16, 8);                                                \
+            else if (g == 4) CALL(BMT_DT_BF16, 4);                                           \
+            else CALL(BMT_DT_BF16, 1);                                                       \
+        } else {                                                                             \
+            if (g == 8) CALL(BMT_DT_F16, 8);                                                 \
+            else if (g == 4) CALL(BMT_DT_F16, 4);                                            \
+            else CALL(BMT_DT_F16, 1);                                                        \
+        }                                                                                    \
+    } while (0)
+
+inline bool known_dtype(int d) { return d == BMT_DT_F32 || d == BMT_DT_BF16 || d == BMT_DT_F16; }
+
+}  // namespace
+
+extern "C" int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, void* out, int64_t N, int D, int V, int dtype, float scale, void* stream) {
+    BMT_CHECK_ARG(known_dtype(dtype) && N >= 0 && D > 0 && V > 0 && ldw >= D, "bmt_embedding: bad args (dtype %d, D %d, V %d)", dtype, D, V);
+    if (N == 0) return BMT_OK;
+    BMT_CHECK_ARG(ids && W && out, "bmt_embedding: null pointer");
+    const int es = dtype == BMT_DT_F32 ? 4 : 2, g = cols_of(es, D, W, ldw, out, D), ncb = bmt_cdiv(D, 64 * g);
+    const int tpw = N >= 16384 ? 4 : 1;      // enough waves to fill the chip: four tokens' loads in flight in each
+    const int64_t tasks = (N + tpw - 1) / tpw * ncb, grid = (tasks + 3) / 4;
+    BMT_CHECK_ARG(grid <= 0x7fffffff, "bmt_embedding: too many tokens");
+#define BMT_CALL(DT, G)                                                                                                                                       \
+    do {                                                                                                                                                      \
+        if (tpw == 4) hipLaunchKernelGGL((embed_kernel<DT, G, 4>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, ids, (const char*)W, ldw, (char*)out, N, D, V, \
+                                         scale, ncb, tasks);                                                                                                  \
+        else hipLaunchKernelGGL((embed_kernel<DT, G, 1>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, ids, (const char*)W, ldw, (char*)out, N, D, V, scale,   \
+                                ncb, tasks);                                                                                                                  \
+    } while (0)
+    BMT_EMB_BY(dtype, g, BMT_CALL);
+#undef BMT_CALL
+    BMT_CHECK_LAUNCH("bmt_embedding");
+    return BMT_OK;
+}
+
+extern "C" int64_t bmt_embedding_bwd_ws_bytes(int64_t N, int D, int V) {
+    if (N < 0 || N > 0x7fffffff - 64 || D <= 0 || V <= 0) return 0;
+    const int64_t chunks = (N + EMB_LONG - 1) / EMB_LONG;
+    return round16(((int64_t)V + 1) * 4) + 2 * round16(N * 4) + (N > EMB_LONG ? 2 * chunks * emb_ld(D) * 4 : 0);
+}
+
+extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t ld, int64_t N, int D, int V, int dtype, float scale, int64_t pad_idx, void* dW, float* into,
+                                 int64_t ldw, void* ws, int64_t ws_bytes, void* stream) {
+    BMT_CHECK_ARG(known_dtype(dtype) && N >= 0 && N <= 0x7fffffff - 64 && D > 0 && V > 0 && ldw >= D && ld >= 0, "bmt_embedding_bwd: bad args (dtype %d, D %d, V %d)", dtype, D, V);
+    BMT_CHECK_ARG((dW != nullptr) != (into != nullptr), "bmt_embedding_bwd: give either dW or the buffer to add to");
+    BMT_CHECK_ARG(!into || dtype == BMT_DT_F32, "bmt_embedding_bwd: only fp32 gradients are added to a buffer");
+    BMT_CHECK_ARG(ws && ws_bytes >= bmt_embedding_bwd_ws_bytes(N, D, V) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0,
+                  "bmt_embedding_bwd: workspace of %lld bytes is too small or not aligned", (long long)ws_bytes);
+    BMT_CHECK_ARG((ids && dout) || N == 0, "bmt_embedding_bwd: null pointer");
+    if (N == 0 && into) return BMT_OK;
+    hipStream_t st = (hipStream_t)stream;
+    int* offsets = (int*)ws;
+    int* order = (int*)((char*)ws + round16(((int64_t)V + 1) * 4));
+    int* token = (int*)((char*)order + round16(N * 4));
+    float* part = (float*)((char*)token + round16(N * 4));
+    const int es = dtype == BMT_DT_F32 ? 4 : 2;
+    const int g = cols_of(es, D, dout, ld, into ? (void*)into : dW, ldw), ncb = bmt_cdiv(D, 64 * g);
+    const int chunks = N > EMB_LONG ? bmt_cdiv(N, EMB_LONG) : 0;      // (fewer positions than that: no token is frequent)
+    const int64_t grid = (int64_t)chunks * ncb + ((int64_t)V * ncb + 3) / 4;
+    const int64_t ldp = emb_ld(D);
+    BMT_CHECK_ARG(grid <= 0x7fffffff, "bmt_embedding_bwd: vocabulary too large");
+    const int nb = bins_for(V), groups = bmt_cdiv(V, nb);
+    const size_t lds = (size_t)16 * nb * sizeof(int);
+#define BMT_ORDER(K) hipLaunchKernelGGL((embed_order_kernel<K>), dim3(groups), dim3(1024), lds, st, ids, N, V, pad_idx, nb, offsets, order, token)
+    if (N <= 1024) BMT_ORDER(1);
+    else if (N <= 4096) BMT_ORDER(4);
+    else if (N <= 16384) BMT_ORDER(16);
+    else if (N <= 65536) BMT_ORDER(64);
+    else BMT_ORDER(0);
+#undef BMT_ORDER
+#define BMT_CALL(DT, G)                                                                                                                                      \
+    do {                                                                                                                                                     \
+        hipLaunchKernelGGL((embed_sum_kernel<DT, G>), dim3((unsigned)grid), dim3(256), 0, st, (const char*)dout, ld, offsets, order, token, part, ldp, (char*)dW, into, ldw, \
+                           D, V, scale, chunks, ncb);                                                                                                        \
+        if (chunks) hipLaunchKernelGGL((embed_join_kernel<DT, G>), dim3((unsigned)(chunks * ncb)), dim3(256), 0, st, offsets, token, part, ldp, (char*)dW, into, ldw, D, V,  \
+                                       scale, ncb);                                                                                                          \
+    } while (0)
+    BMT_EMB_BY(dtype, g, BMT_CALL);
+#undef BMT_CALL
+    BMT_CHECK_LAUNCH("bmt_embedding_bwd");
+    return BMT_OK;
+}

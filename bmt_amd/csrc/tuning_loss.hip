@@ -1,0 +1,705 @@
+// Losses that tune a caption model on its own samples, from the logits, with their gradients:
+//   token log-probability   lp_r = x_r[id_r] - max_c x_rc - log sum_c exp(x_rc - max)         (rows r = (sequence b, position t))
+//   clipped policy loss     rho = exp(lp - old), l_r = -min(rho A, clip(rho, 1 - lo, 1 + hi) A) + beta (exp(ref - lp) - (ref - lp) - 1)
+//   paired preference loss  S_b = sum_t lp, r_b = beta (S_b - ref_b), z = r_b - r_{b+P}, loss = mean -(1 - ls) log sig(z) - ls log sig(-z)
+// All three have d loss / d x_rc = w_r (1[c = id_r] - exp(x_rc - max) / s) with ONE number w_r per row.
+// Bound: HBM -- about 15 fp32 operations per logit against 4 - 8 bytes moved.  The policy loss needs nothing from other rows but their count, so
+// a row stays in the registers of its workgroup from the maximum to the gradient: every logit is read once and every gradient written once.  The
+// preference loss needs the whole pair before any gradient: its logits are read twice.
+// Numerics: maxima and exponentials in fp32, a thread's partial sums in fp32 (at most a few hundred terms), across threads and everything that
+// belongs to a row or a sequence in 64 bits; 16-bit gradients are rounded once.  No atomics: results do not depend on the schedule.
+// Rows that do not count (mask 0, or the padding id) are not read; their gradient rows are written as zeros.
+#include "common.h"
+
+namespace {
+
+template <int DT>
+struct Elem;      // BMT_DT_*: bytes per element, elements per 16-byte granule, granule <-> floats
+template <>
+struct Elem<BMT_DT_F32> {
+    static constexpr int B = 4, G = 4;
+    static __device__ __forceinline__ uint32_t lowest() { return 0xff800000u; }
+    static __device__ __forceinline__ void get(const u32x4& v, float (&x)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(v[j]);
+    }
+    static __device__ __forceinline__ u32x4 put(const float (&x)[4]) {
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(x[j]);
+        return v;
+    }
+    static __device__ __forceinline__ float get1(const char* p) { return *reinterpret_cast<const float*>(p); }
+};
+template <>
+struct Elem<BMT_DT_BF16> {
+    static constexpr int B = 2, G = 8;
+    static __device__ __forceinline__ uint32_t lowest() { return 0xff80ff80u; }
+    static __device__ __forceinline__ void get(const u32x4& v, float (&x)[8]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = __uint_as_float(v[j] << 16);
+            x[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 put(const float (&x)[8]) {
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
+        return v;
+    }
+    static __device__ __forceinline__ float get1(const char* p) { return bf_bits2f(*reinterpret_cast<const uint16_t*>(p)); }
+};
+template <>
+struct Elem<BMT_DT_F16> {
+    static constexpr int B = 2, G = 8;
+    static __device__ __forceinline__ uint32_t lowest() { return 0xfc00fc00u; }
+    static __device__ __forceinline__ void get(const u32x4& v, float (&x)[8]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = h_bits2f(v[j] & 0xffffu);
+            x[2 * j + 1] = h_bits2f(v[j] >> 16);
+        }
+    }
+    static __device__ __forceinline__ u32x4 put(const float (&x)[8]) {
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = pack_h2(x[2 * j], x[2 * j + 1]);
+        return v;
+    }
+    static __device__ __forceinline__ float get1(const char* p) { return h_bits2f(*reinterpret_cast<const uint16_t*>(p)); }
+};
+
+// the (B, T) rows of a call: logits with two row strides, ids and an optional mask with theirs (all strides in elements)
+struct Rows {
+    const char* x;
+    int64_t sb, st;
+    int T, V;
+    const int64_t* id;
+    int64_t ib, it;
+    const uint8_t* mask;
+    int64_t mb, mt;
+    int64_t pad;
+};
+struct PolicyIn {
+    const float *old, *ref, *adv;      // old NULL: the ratio is 1 (on-policy); ref NULL: no KL term
+    int64_t ob, ot, rb, rt, ab, at;
+    float lo, hi, beta;
+    int reduction;                     // 0 sum, 1 mean over the rows that count, 2 mean over sequences of their means
+    int B;
+    const int* counts;                 // [B] rows that count per sequence, [B] their total
+};
+
+__device__ __forceinline__ bool row_counts(const Rows& q, int b, int t, int64_t id) {
+    return id != q.pad && (q.mask == nullptr || q.mask[b * q.mb + t * q.mt] != 0);
+}
+
+// A row as 16-byte granules of memory: the first one starts at or below the row's first element, so that vector accesses are aligned for every
+// start and every odd V; the elements of the two edge granules that are not the row's are never touched
+template <int DT>
+struct Row {
+    using E = Elem<DT>;
+    char* base;      // 16-byte aligned
+    int phase, end;  // the row's elements are [phase, end) from base
+    __device__ __forceinline__ Row(const char* p, int V) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+        base = reinterpret_cast<char*>(a & ~(uintptr_t)15);
+        phase = (int)(a & 15) / E::B;
+        end = phase + V;
+    }
+    __device__ __forceinline__ int granules() const { return (end + E::G - 1) / E::G; }
+    __device__ __forceinline__ bool inner(int k) const { return k * E::G >= phase && (k + 1) * E::G <= end; }
+    __device__ __forceinline__ u32x4 load(int k) const {
+        const char* p = base + (int64_t)k * 16;
+        if (inner(k)) return *reinterpret_cast<const u32x4*>(p);
+        const uint32_t l = E::lowest();
+        u32x4 v = {l, l, l, l};      // -inf: adds nothing to the maximum nor to the sum
+#pragma unroll
+        for (int j = 0; j < E::G; ++j) {
+            const int e = k * E::G + j;
+            if (e >= phase && e < end) {
+                if constexpr (E::B == 4) v[j] = *reinterpret_cast<const uint32_t*>(p + 4 * j);
+                else {
+                    const uint32_t h = *reinterpret_cast<const uint16_t*>(p + 2 * j);
+                    v[j / 2] = (j & 1) ? ((v[j / 2] & 0xffffu) | (h << 16)) : ((v[j / 2] & 0xffff0000u) | h);
+                }
+            }
+        }
+        return v;
+    }
+    __device__ __forceinline__ void store_elements(int k, const u32x4& v, char* row) const {      // row: where element `phase` goes
+#pragma unroll
+        for (int j = 0; j < E::G; ++j) {
+            const int e = k * E::G + j;
+            if (e >= phase && e < end) {
+                if constexpr (E::B == 4) *reinterpret_cast<uint32_t*>(row + (int64_t)(e - phase) * 4) = v[j];
+                else *reinterpret_cast<uint16_t*>(row + (int64_t)(e - phase) * 2) = (uint16_t)(v[j / 2] >> ((j & 1) * 16));
+            }
+        }
+    }
+};
+
+// writes granule k of the row to `out` (same phase: 16-byte stores; another one: element by element)
+template <int DT>
+__device__ __forceinline__ void put_granule(const Row<DT>& row, int k, const u32x4& v, char* out, bool same) {
+    if (same && row.inner(k)) *reinterpret_cast<u32x4*>(out + ((int64_t)k * Elem<DT>::G - row.phase) * Elem<DT>::B) = v;
+    else row.store_elements(k, v, out);
+}
+__device__ __forceinline__ bool same_phase(const char* a, const char* b) { return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0; }
+
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+template <int NT>
+__device__ __forceinline__ float group_max(float v, float* red) {
+    v = wave_max(v);
+    if constexpr (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float m = red[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) m = fmaxf(m, red[i]);
+    return m;
+}
+template <int NT>
+__device__ __forceinline__ double group_sum(double v, double* red) {
+    v = wave_sum_f64(v);
+    if constexpr (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = red[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) s += red[i];
+    return s;
+}
+
+// everything a policy row adds to the loss, in 64 bits: the differences of log-probabilities are small beside the values they come from, and the
+// KL term is second order in them.  Returns w_r; terms[0..2] = the row's share of the loss, its KL, whether the clip took its gradient
+__device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, double lp, double* terms) {
+    const double A = p.adv[b * p.ab + t * p.at];
+    const double rho = p.old ? exp(lp - (double)p.old[b * p.ob + t * p.ot]) : exp(lp - lp);      // (lp - lp: NaN stays NaN)
+    const double u = rho * A, c = fmin(fmax(rho, 1.0 - (double)p.lo), 1.0 + (double)p.hi) * A;
+    const bool clipped = u > c;
+    double loss = clipped ? -c : -u, w = clipped ? 0.0 : -u, kl = 0.0;
+    if (p.ref) {
+        const double d = (double)p.ref[b * p.rb + t * p.rt] - lp, em = expm1(d);
+        kl = em - d;
+        loss += (double)p.beta * kl;
+        w -= (double)p.beta * em;
+    }
+    double norm = 1.0;
+    if (p.reduction == 1) norm = 1.0 / (double)max(p.counts[p.B], 1);
+    else if (p.reduction == 2) norm = 1.0 / ((double)p.B * (double)max(p.counts[b], 1));
+    terms[0] = loss * norm;
+    terms[1] = kl;
+    terms[2] = clipped ? 1.0 : 0.0;
+    return (float)(w * norm);
+}
+
+// ---------------------------------------------------------------- rows that count, per sequence and in all (one workgroup)
+// a wave per sequence, or -- short sequences -- a thread per sequence: 64 lanes would wait on a handful of loads
+__global__ __launch_bounds__(1024) void count_rows_kernel(Rows q, int B, int* __restrict__ counts) {
+    __shared__ int red[16];
+    int total = 0;
+    if (q.T < 32) {
+        for (int b = threadIdx.x; b < B; b += 1024) {
+            int n = 0;
+            for (int t = 0; t < q.T; ++t) n += row_counts(q, b, t, q.id[b * q.ib + t * q.it]);
+            counts[b] = n;
+            total += n;
+        }
+    } else {
+        for (int b = threadIdx.x >> 6; b < B; b += 16) {
+            int n = 0;
+            for (int t = threadIdx.x & 63; t < q.T; t += 64) n += row_counts(q, b, t, q.id[b * q.ib + t * q.it]);
+            total += n;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+            if ((threadIdx.x & 63) == 0) counts[b] = n;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) total += red[i];
+        counts[B] = total;
+    }
+}
+
+// ---------------------------------------------------------------- forward: statistics and log-probability of every row, any V
+// One sweep with a running maximum and sum per thread.  stats[r] = {max, 1 / sum} for the gradient kernel (0, 0 where the row does not count).
+template <int DT, int NT, bool POLICY>
+__global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float* __restrict__ logp, float2* __restrict__ stats, float* __restrict__ w,
+                                                        double* __restrict__ terms, int64_t rows) {
+    using E = Elem<DT>;
+    constexpr int U = 4;
+    __shared__ float redf[NT / 64];
+    __shared__ double redd[NT / 64];
+    const int64_t r = blockIdx.x;
+    const int b = (int)(r / q.T), t = (int)(r % q.T);
+    const int64_t id = q.id[b * q.ib + t * q.it];
+    if (!row_counts(q, b, t, id)) {
+        if (threadIdx.x == 0) {
+            logp[r] = 0.f;
+            if (stats) stats[r] = make_float2(0.f, 0.f);
+            if constexpr (POLICY) {
+                w[r] = 0.f;
+                terms[r] = terms[rows + r] = terms[2 * rows + r] = 0.0;
+            }
+        }
+        return;
+    }
+    const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
+    const Row<DT> row(xr, q.V);
+    const int n = row.granules();
+    float xt = __builtin_nanf("");      // an id outside the vocabulary has no log-probability
+    if (threadIdx.x == 0 && id >= 0 && id < q.V) xt = E::get1(xr + id * E::B);
+    float m = -__builtin_huge_valf(), s = 0.f;
+    for (int k0 = threadIdx.x; k0 < n; k0 += NT * U) {
+        u32x4 v[U];
+        const uint32_t l = E::lowest();
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            v[i] = u32x4{l, l, l, l};
+            if (k0 + i * NT < n) v[i] = row.load(k0 + i * NT);
+        }
+        float x[U][E::G], bm = -__builtin_huge_valf();
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            E::get(v[i], x[i]);
+#pragma unroll
+            for (int j = 0; j < E::G; ++j) bm = fmaxf(bm, x[i][j]);
+        }
+        const float mn = fmaxf(m, bm), ms = mn == -__builtin_huge_valf() ? 0.f : mn;      // (nothing but -inf so far: the sum stays 0)
+        s *= __expf(m - ms);
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int j = 0; j < E::G; ++j) a += __expf(x[i][j] - ms);
+        s += a;
+        m = mn;
+    }
+    const float M = group_max<NT>(m, redf);
+    const double S = group_sum<NT>(m == -__builtin_huge_valf() ? (double)s : (double)s * (double)__expf(m - M), redd);
+    if (threadIdx.x == 0) {
+        const double lp = ((double)xt - (double)M) - log(S);
+        logp[r] = (float)lp;
+        if (stats) stats[r] = make_float2(M, (float)(1.0 / S));
+        if constexpr (POLICY) {
+            double tr[3];
+            w[r] = policy_row(p, b, t, lp, tr);
+            terms[r] = tr[0];
+            terms[rows + r] = tr[1];
+            terms[2 * rows + r] = tr[2];
+        }
+    }
+}
+
+// ---------------------------------------------------------------- policy loss: statistics, loss terms and gradient of a row in one visit
+// The row (at most NT * NV granules) stays in registers as it was loaded.
+template <int DT, int NT, int NV>
+__global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, char* __restrict__ dx, int64_t db, int64_t dt, float* __restrict__ logp,
+                                                          float2* __restrict__ stats, float* __restrict__ w, double* __restrict__ terms, int64_t rows) {
+    using E = Elem<DT>;
+    __shared__ float redf[NT / 64];
+    __shared__ double redd[NT / 64];
+    __shared__ float wc[2];
+    const int64_t r = blockIdx.x;
+    const int b = (int)(r / q.T), t = (int)(r % q.T);
+    const int64_t id = q.id[b * q.ib + t * q.it];
+    const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
+    char* dr = dx + (b * db + t * dt) * E::B;
+    if (!row_counts(q, b, t, id)) {
+        const Row<DT> o(dr, q.V);
+        for (int k = threadIdx.x, n = o.granules(); k < n; k += NT) put_granule<DT>(o, k, u32x4{0, 0, 0, 0}, dr, true);
+        if (threadIdx.x == 0) {
+            logp[r] = 0.f;
+            stats[r] = make_float2(0.f, 0.f);
+            w[r] = 0.f;
+            terms[r] = terms[rows + r] = terms[2 * rows + r] = 0.0;
+        }
+        return;
+    }
+    const Row<DT> row(xr, q.V);
+    const int n = row.granules();
+    float xt = __builtin_nanf("");      // an id outside the vocabulary has no log-probability
+    if (threadIdx.x == 0 && id >= 0 && id < q.V) xt = E::get1(xr + id * E::B);
+    u32x4 v[NV];
+    const uint32_t l = E::lowest();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        v[i] = u32x4{l, l, l, l};
+        if ((int)threadIdx.x + NT * i < n) v[i] = row.load(threadIdx.x + NT * i);
+    }
+    float m = -__builtin_huge_valf();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float x[E::G];
+        E::get(v[i], x);
+#pragma unroll
+        for (int j = 0; j < E::G; ++j) m = fmaxf(m, x[j]);
+    }
+    m = group_max<NT>(m, redf);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (NT * i < n) {      // (whole slots behind the row's end)
+            float x[E::G], a = 0.f;
+            E::get(v[i], x);
+#pragma unroll
+            for (int j = 0; j < E::G; ++j) a += __expf(x[j] - m);
+            s += a;
+        }
+    }
+    const double S = group_sum<NT>((double)s, redd);
+    if (threadIdx.x == 0) {
+        const double lp = ((double)xt - (double)m) - log(S);
+        double tr[3];
+        const float wr = policy_row(p, b, t, lp, tr);
+        const float is = (float)(1.0 / S);
+        wc[0] = wr;
+        wc[1] = is;
+        logp[r] = (float)lp;
+        stats[r] = make_float2(m, is);
+        w[r] = wr;
+        terms[r] = tr[0];
+        terms[rows + r] = tr[1];
+        terms[2 * rows + r] = tr[2];
+    }
+    __syncthreads();
+    const float wr = wc[0], c = -wr * wc[1];
+    const int kt = (int)((row.phase + id) / E::G), jt = (int)((row.phase + id) % E::G);      // (outside the vocabulary: wr is NaN everywhere)
+    const bool same = same_phase(xr, dr);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int k = threadIdx.x + NT * i;
+        if (k < n) {
+            float x[E::G];
+            E::get(v[i], x);
+#pragma unroll
+            for (int j = 0; j < E::G; ++j) x[j] = __expf(x[j] - m) * c;
+            if (k == kt) {
+#pragma unroll
+                for (int j = 0; j < E::G; ++j)
+                    if (j == jt) x[j] += wr;
+            }
+            put_granule<DT>(row, k, E::put(x), dr, same);
+        }
+    }
+}
+
+// loss[0] = sum of the rows' shares, info[0] = mean KL, info[1] = share of rows whose gradient the clip took (means over the rows that count)
+__global__ __launch_bounds__(1024) void policy_finish_kernel(const double* __restrict__ terms, int64_t rows, const int* __restrict__ total, float* __restrict__ loss,
+                                                              float* __restrict__ info) {
+    __shared__ double red[3][16];
+    double a[3] = {0.0, 0.0, 0.0};
+    for (int64_t r = threadIdx.x; r < rows; r += 1024)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) a[k] += terms[k * rows + r];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        a[k] = wave_sum_f64(a[k]);
+        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = a[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        double v = 0.0;
+        for (int i = 0; i < 16; ++i) v += red[threadIdx.x][i];
+        const double n = (double)max(total[0], 1);
+        if (threadIdx.x == 0) loss[0] = (float)v;
+        else info[threadIdx.x - 1] = (float)(v / n);
+    }
+}
+
+// ---------------------------------------------------------------- gradient from saved statistics: dx = g w_r (1[c = id] - exp(x - max) / sum)
+// g (optional): the loss's upstream gradient.  once: dx already holds the gradient for g = 1 -- nothing to do then
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __restrict__ stats, const float* __restrict__ w, int64_t wb, int64_t wt,
+                                                         const float* __restrict__ g, int once, char* __restrict__ dx, int64_t db, int64_t dt, int64_t rows) {
+    using E = Elem<DT>;
+    const float gs = g ? g[0] : 1.f;
+    if (once && gs == 1.f) return;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const int b = (int)(r / q.T), t = (int)(r % q.T);
+        const int64_t id = q.id[b * q.ib + t * q.it];
+        const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
+        char* dr = dx + (b * db + t * dt) * E::B;
+        if (!row_counts(q, b, t, id)) {
+            const Row<DT> o(dr, q.V);
+            for (int k = threadIdx.x, n = o.granules(); k < n; k += NT) put_granule<DT>(o, k, u32x4{0, 0, 0, 0}, dr, true);
+            continue;
+        }
+        const Row<DT> row(xr, q.V);
+        const int n = row.granules();
+        const float2 st = stats[r];
+        const float wr = w[b * wb + t * wt] * gs, m = st.x, c = -wr * st.y;
+        const int kt = (int)((row.phase + id) / E::G), jt = (int)((row.phase + id) % E::G);
+        const bool same = same_phase(xr, dr);
+        for (int k = threadIdx.x; k < n; k += NT) {
+            float x[E::G];
+            E::get(row.load(k), x);
+#pragma unroll
+            for (int j = 0; j < E::G; ++j) x[j] = __expf(x[j] - m) * c;
+            if (k == kt) {
+#pragma unroll
+                for (int j = 0; j < E::G; ++j)
+                    if (j == jt) x[j] += wr;
+            }
+            put_granule<DT>(row, k, E::put(x), dr, same);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- preference loss from the rows' log-probabilities: a wave per pair
+__device__ __forceinline__ double softplus64(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+__device__ __forceinline__ double sigmoid64(double x) { return 1.0 / (1.0 + exp(-x)); }
+
+__global__ __launch_bounds__(1024) void preference_pairs_kernel(const float* __restrict__ logp, const float2* __restrict__ stats, int P, int T, const float* __restrict__ ref,
+                                                                 int64_t rs, float beta, float smoothing, int mean, float* __restrict__ rewards, float* __restrict__ w,
+                                                                 double* __restrict__ pair_loss, float* __restrict__ loss) {
+    __shared__ double red[16];
+    const int lane = threadIdx.x & 63;
+    double acc = 0.0;
+    for (int i = blockIdx.x * 16 + (threadIdx.x >> 6); i < P; i += gridDim.x * 16) {
+        double S[2], len[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t r0 = (int64_t)(i + h * P) * T;
+            double a = 0.0, c = 0.0;
+            for (int t = lane; t < T; t += 64) {
+                a += (double)logp[r0 + t];
+                c += stats[r0 + t].y == 0.f ? 0.0 : 1.0;      // (a row that counts has a finite sum)
+            }
+            S[h] = wave_sum_f64(a);
+            len[h] = fmax(wave_sum_f64(c), 1.0);
+        }
+        const double i0 = mean ? 1.0 / len[0] : 1.0, i1 = mean ? 1.0 / len[1] : 1.0;
+        const double r0 = (double)beta * (S[0] * i0 - (double)ref[(int64_t)i * rs]), r1 = (double)beta * (S[1] * i1 - (double)ref[(int64_t)(i + P) * rs]);
+        const double z = r0 - r1, ls = (double)smoothing;
+        double l = (1.0 - ls) * softplus64(-z), d = (1.0 - ls) * sigmoid64(-z);
+        if (ls != 0.0) {      // (0 * inf)
+            l += ls * softplus64(z);
+            d -= ls * sigmoid64(z);
+        }
+        d *= -(double)beta / (double)P;
+        if (lane == 0) {
+            rewards[i] = (float)r0;
+            rewards[i + P] = (float)r1;
+            if (w) {
+                w[i] = (float)(d * i0);
+                w[i + P] = (float)(-d * i1);
+            }
+            if (pair_loss) pair_loss[i] = l / (double)P;
+        }
+        acc += l / (double)P;
+    }
+    if (gridDim.x > 1) return;      // (sum_f64_kernel adds pair_loss)
+    if (lane == 0) red[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; ++k) acc += red[k];
+        loss[0] = (float)acc;
+    }
+}
+
+__global__ __launch_bounds__(1024) void sum_f64_kernel(const double* __restrict__ v, int64_t n, float* __restrict__ out) {
+    __shared__ double red[16];
+    double a = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) a += v[i];
+    a = group_sum<1024>(a, red);
+    if (threadIdx.x == 0) out[0] = (float)a;
+}
+
+inline int elem_bytes(int dtype) { return dtype == BMT_DT_F32 ? 4 : 2; }
+
+int check_rows(const char* who, const void* x, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* id) {
+    BMT_CHECK_ARG(dtype == BMT_DT_F32 || dtype == BMT_DT_BF16 || dtype == BMT_DT_F16, "%s: unknown dtype %d", who, dtype);
+    BMT_CHECK_ARG(B >= 0 && T >= 0 && V > 0 && V <= (1 << 30) && sb >= 0 && st >= 0, "%s: bad sizes B=%d T=%d V=%d", who, B, T, V);
+    BMT_CHECK_ARG((int64_t)B * T <= 0x7fffffff, "%s: %d x %d rows are more than a grid holds", who, B, T);
+    BMT_CHECK_ARG((x && id) || (int64_t)B * T == 0, "%s: null pointer", who);
+    BMT_CHECK_ARG((reinterpret_cast<uintptr_t>(x) & (elem_bytes(dtype) - 1)) == 0, "%s: logits are not aligned to their elements", who);
+    return BMT_OK;
+}
+
+// threads per row: about 4 granules each are in flight in one batch, and a few rows cannot fill 256 CUs with small workgroups
+inline int threads_for(int64_t rows, int64_t granules) {
+    if (granules <= 256) return 64;
+    return rows < 512 && granules > 1024 ? 1024 : 256;
+}
+
+template <int DT>
+void launch_logp(const Rows& q, const PolicyIn* p, float* logp, float2* stats, float* w, double* terms, int64_t rows, hipStream_t st) {
+    const int nt = threads_for(rows, ((int64_t)q.V + Elem<DT>::G - 1) / Elem<DT>::G);
+    const PolicyIn none = {};
+#define BMT_ROWS(NT)                                                                                                                               \
+    do {                                                                                                                                           \
+        if (p) hipLaunchKernelGGL((logp_rows_kernel<DT, NT, true>), dim3((unsigned)rows), dim3(NT), 0, st, q, *p, logp, stats, w, terms, rows);      \
+        else hipLaunchKernelGGL((logp_rows_kernel<DT, NT, false>), dim3((unsigned)rows), dim3(NT), 0, st, q, none, logp, stats, w, terms, rows);     \
+    } while (0)
+    if (nt == 64) BMT_ROWS(64);
+    else if (nt == 256) BMT_ROWS(256);
+    else BMT_ROWS(1024);
+#undef BMT_ROWS
+}
+
+template <int DT>
+void launch_grad(const Rows& q, const float2* stats, const float* w, int64_t wb, int64_t wt, const float* g, int once, void* dx, int64_t db, int64_t dt, int64_t rows,
+                 hipStream_t st) {
+    const int nt = threads_for(rows, ((int64_t)q.V + Elem<DT>::G - 1) / Elem<DT>::G);
+    const unsigned grid = (unsigned)(once && rows > 2048 ? 2048 : rows);      // (once: usually every workgroup ends at its first instruction)
+#define BMT_GRAD(NT) hipLaunchKernelGGL((logit_grad_kernel<DT, NT>), dim3(grid), dim3(NT), 0, st, q, stats, w, wb, wt, g, once, (char*)dx, db, dt, rows)
+    if (nt == 64) BMT_GRAD(64);
+    else if (nt == 256) BMT_GRAD(256);
+    else BMT_GRAD(1024);
+#undef BMT_GRAD
+}
+
+// the fused form where a row fits the registers of a workgroup; false: it does not
+template <int DT>
+bool launch_policy(const Rows& q, const PolicyIn& p, void* dx, int64_t db, int64_t dt, float* logp, float2* stats, float* w, double* terms, int64_t rows, hipStream_t st) {
+    const int64_t n = ((int64_t)q.V + Elem<DT>::G - 1) / Elem<DT>::G + 1;      // (+ 1: a row that starts inside a granule)
+#define BMT_POL(NT, NV)                                                                                                                                       \
+    do {                                                                                                                                                      \
+        hipLaunchKernelGGL((policy_rows_kernel<DT, NT, NV>), dim3((unsigned)rows), dim3(NT), 0, st, q, p, (char*)dx, db, dt, logp, stats, w, terms, rows);     \
+        return true;                                                                                                                                          \
+    } while (0)
+    const int nt = threads_for(rows, n - 1);
+    if (nt == 64 && n <= 64 * 2) BMT_POL(64, 2);
+    if (nt == 64) BMT_POL(64, 5);
+    if (nt == 256 && n <= 256 * 4) BMT_POL(256, 4);
+    if (nt == 256 && n <= 256 * 8) BMT_POL(256, 8);
+    if (nt == 256 && n <= 256 * 12) BMT_POL(256, 12);
+    if (nt == 256 && n <= 256 * 16) BMT_POL(256, 16);
+    if (n <= 1024 * 4) BMT_POL(1024, 4);
+    if (n <= 1024 * 8) BMT_POL(1024, 8);
+    if (n <= 1024 * 16) BMT_POL(1024, 16);
+#undef BMT_POL
+    return false;
+}
+
+#define BMT_BY_DTYPE(dtype, CALL)                       \
+    do {                                                \
+        if (dtype == BMT_DT_F32) CALL(BMT_DT_F32);      \
+        else if (dtype == BMT_DT_BF16) CALL(BMT_DT_BF16); \
+        else CALL(BMT_DT_F16);                          \
+    } while (0)
+
+}  // namespace
+
+extern "C" int bmt_logp_rows(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
+                             const uint8_t* mask, int64_t mb, int64_t mt, int64_t pad_idx, float* logp, float* stats, void* stream) {
+    const int rc = check_rows("bmt_logp_rows", logits, dtype, sb, st, B, T, V, ids);
+    if (rc != BMT_OK) return rc;
+    const int64_t rows = (int64_t)B * T;
+    if (rows == 0) return BMT_OK;
+    BMT_CHECK_ARG(logp, "bmt_logp_rows: null pointer");
+    const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
+#define BMT_CALL(DT) launch_logp<DT>(q, nullptr, logp, (float2*)stats, nullptr, nullptr, rows, (hipStream_t)stream)
+    BMT_BY_DTYPE(dtype, BMT_CALL);
+#undef BMT_CALL
+    BMT_CHECK_LAUNCH("bmt_logp_rows");
+    return BMT_OK;
+}
+
+extern "C" int bmt_logit_grad(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
+                              const uint8_t* mask, int64_t mb, int64_t mt, int64_t pad_idx, const float* stats, const float* w, int64_t wb, int64_t wt,
+                              const float* gscale_dev, int once, void* dlogits, int64_t db, int64_t dt, void* stream) {
+    const int rc = check_rows("bmt_logit_grad", logits, dtype, sb, st, B, T, V, ids);
+    if (rc != BMT_OK) return rc;
+    const int64_t rows = (int64_t)B * T;
+    if (rows == 0) return BMT_OK;
+    BMT_CHECK_ARG(stats && w && dlogits && db >= 0 && dt >= 0, "bmt_logit_grad: null pointer");
+    BMT_CHECK_ARG((reinterpret_cast<uintptr_t>(dlogits) & (elem_bytes(dtype) - 1)) == 0, "bmt_logit_grad: the gradient is not aligned to its elements");
+    const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
+#define BMT_CALL(DT) launch_grad<DT>(q, (const float2*)stats, w, wb, wt, gscale_dev, once, dlogits, db, dt, rows, (hipStream_t)stream)
+    BMT_BY_DTYPE(dtype, BMT_CALL);
+#undef BMT_CALL
+    BMT_CHECK_LAUNCH("bmt_logit_grad");
+    return BMT_OK;
+}
+
+extern "C" int64_t bmt_policy_ws_bytes(int B, int T) {
+    if (B < 0 || T < 0) return 0;
+    return (int64_t)B * T * (3 * 8 + 3 * 4) + ((int64_t)B + 1) * 4;
+}
+
+extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
+                               const uint8_t* mask, int64_t mb, int64_t mt, int64_t pad_idx, const float* old_logp, int64_t ob, int64_t ot, const float* ref_logp,
+                               int64_t rb, int64_t rt, const float* adv, int64_t ab, int64_t at, float clip_low, float clip_high, float kl_coef, int reduction,
+                               float* loss, float* info, float* logp, void* ws, int64_t ws_bytes, void* dlogits, int64_t db, int64_t dt, void* stream) {
+    const int rc = check_rows("bmt_policy_loss", logits, dtype, sb, st, B, T, V, ids);
+    if (rc != BMT_OK) return rc;
+    const int64_t rows = (int64_t)B * T;
+    BMT_CHECK_ARG(rows > 0, "bmt_policy_loss: no rows");
+    BMT_CHECK_ARG(adv && loss && info && logp && ws, "bmt_policy_loss: null pointer");
+    BMT_CHECK_ARG(reduction >= 0 && reduction <= 2, "bmt_policy_loss: unknown reduction %d", reduction);
+    BMT_CHECK_ARG(clip_low >= 0.f && clip_high >= 0.f, "bmt_policy_loss: negative clip range");
+    BMT_CHECK_ARG(ws_bytes >= bmt_policy_ws_bytes(B, T) && (reinterpret_cast<uintptr_t>(ws) & 7) == 0, "bmt_policy_loss: workspace of %lld bytes is too small or not aligned",
+                  (long long)ws_bytes);
+    BMT_CHECK_ARG(!dlogits || (db >= 0 && dt >= 0 && (reinterpret_cast<uintptr_t>(dlogits) & (elem_bytes(dtype) - 1)) == 0), "bmt_policy_loss: bad gradient layout");
+    hipStream_t s = (hipStream_t)stream;
+    // workspace: terms [3][rows] (64-bit) | stats [rows][2] | w [rows] | counts [B + 1]
+    double* terms = (double*)ws;
+    float2* stats = (float2*)(terms + 3 * rows);
+    float* w = (float*)(stats + rows);
+    int* counts = (int*)(w + rows);
+    const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
+    const PolicyIn p = {old_logp, ref_logp, adv, ob, ot, rb, rt, ab, at, clip_low, clip_high, kl_coef, reduction, B, counts};
+    hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, s, q, B, counts);
+    bool done = false;
+#define BMT_CALL(DT) done = launch_policy<DT>(q, p, dlogits, db, dt, logp, stats, w, terms, rows, s)
+    if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
+#undef BMT_CALL
+    if (!done) {      // no gradient wanted, or rows too long for the registers: a second read
+#define BMT_CALL(DT) launch_logp<DT>(q, &p, logp, stats, w, terms, rows, s)
+        BMT_BY_DTYPE(dtype, BMT_CALL);
+#undef BMT_CALL
+#define BMT_CALL(DT) launch_grad<DT>(q, stats, w, T, 1, nullptr, 0, dlogits, db, dt, rows, s)
+        if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
+#undef BMT_CALL
+    }
+    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, s, terms, rows, counts + B, loss, info);
+    BMT_CHECK_LAUNCH("bmt_policy_loss");
+    return BMT_OK;
+}
+
+extern "C" int64_t bmt_preference_ws_bytes(int B, int T) {
+    if (B < 0 || T < 0) return 0;
+    return (int64_t)B * T * (2 * 4 + 4) + (int64_t)B * 4 + 8 + (int64_t)(B / 2) * 8;
+}
+
+extern "C" int bmt_preference_loss(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it, const uint8_t* mask,
+                                   int64_t mb, int64_t mt, int64_t pad_idx, const float* ref_logp, int64_t ref_stride, float beta, float smoothing, int mean_logp, float* loss,
+                                   float* rewards, void* ws, int64_t ws_bytes, void* stream) {
+    const int rc = check_rows("bmt_preference_loss", logits, dtype, sb, st, B, T, V, ids);
+    if (rc != BMT_OK) return rc;
+    const int64_t rows = (int64_t)B * T;
+    BMT_CHECK_ARG(rows > 0 && B % 2 == 0, "bmt_preference_loss: %d sequences are not pairs", B);
+    BMT_CHECK_ARG(ref_logp && loss && rewards && ws, "bmt_preference_loss: null pointer");
+    BMT_CHECK_ARG(smoothing >= 0.f && smoothing <= 1.f, "bmt_preference_loss: smoothing outside [0, 1]");
+    BMT_CHECK_ARG(ws_bytes >= bmt_preference_ws_bytes(B, T) && (reinterpret_cast<uintptr_t>(ws) & 7) == 0,
+                  "bmt_preference_loss: workspace of %lld bytes is too small or not aligned", (long long)ws_bytes);
+    hipStream_t s = (hipStream_t)stream;
+    // workspace: stats [rows][2] | w [B] | logp [rows] | pad to 8 | pair losses [B / 2] (64-bit)
+    float2* stats = (float2*)ws;
+    float* w = (float*)(stats + rows);
+    float* logp = w + B;
+    double* pair = (double*)((char*)ws + (rows * 12 + (int64_t)B * 4 + 7) / 8 * 8);
+    const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
+#define BMT_CALL(DT) launch_logp<DT>(q, nullptr, logp, stats, nullptr, nullptr, rows, s)
+    BMT_BY_DTYPE(dtype, BMT_CALL);
+#undef BMT_CALL
+    const int pairs = B / 2, blocks = pairs <= 128 ? 1 : bmt_cdiv(pairs, 16);      // one workgroup (8 pairs a wave) adds its own losses
+    hipLaunchKernelGGL(preference_pairs_kernel, dim3(blocks), dim3(1024), 0, s, logp, stats, pairs, T, ref_logp, ref_stride, beta, smoothing, mean_logp, rewards, w,
+                       blocks > 1 ? pair : nullptr, loss);
+    if (blocks > 1) hipLaunchKernelGGL(sum_f64_kernel, dim3(1), dim3(1024), 0, s, pair, (int64_t)pairs, loss);
+    BMT_CHECK_LAUNCH("bmt_preference_loss");
+    return BMT_OK;
+}

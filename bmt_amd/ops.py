@@ -3594,3 +3594,321 @@ def mask_from_tokens(trg: torch.Tensor, pad_idx: int, want_src: bool = True, wan
     tm = torch.empty(B, S, S, device=t.device, dtype=torch.uint8) if want_trg else None
     _lib.check(lib.bmt_mask_from_tokens(_p(t), int(pad_idx), _p(src), _p(tm), B, S, _st()), "bmt_mask_from_tokens")
     return (None if src is None else src.view(torch.bool)), (None if tm is None else tm.view(torch.bool))
+
+
+# ----------------------------------------------------------------------------- tuning on sampled captions: losses from logits, embedding
+# (kernels: csrc/tuning_loss.hip, csrc/embedding.hip)
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # BMT_DT_*
+_NO_PAD = -(1 << 63)
+
+
+def _tuning_device(who: str, *tensors) -> torch.device:
+    """the one device all the tensors (None: absent) are on"""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{who}: bmt_amd ops need CUDA/HIP tensors: there is no CPU fallback (use the oracle for CPU checks)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _run_on(dev: torch.device, what: str, fn, *args):
+    """fn(*args, stream) on the current stream of ``dev``, which need not be the current device"""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc != 0:
+        _lib.check(rc, what)
+
+
+def _check_rows(who: str, logits, ids, mask):
+    if logits.dim() != 3 or ids.shape != logits.shape[:2]:
+        raise ValueError(f"{who}: logits (B, T, V) and ids (B, T), not {tuple(logits.shape)} and {tuple(ids.shape)}")
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"{who}: logits of type {logits.dtype} (float32, bfloat16 or float16)")
+    if ids.dtype != torch.int64:
+        raise ValueError(f"{who}: ids of type {ids.dtype} (int64)")
+    if mask is not None and (mask.shape != ids.shape or mask.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"{who}: mask of shape {tuple(mask.shape)} and type {mask.dtype} (a bool or uint8 one of {tuple(ids.shape)})")
+    if logits.shape[2] == 0 or logits.shape[2] > 1 << 30:
+        raise ValueError(f"{who}: a vocabulary of {logits.shape[2]} tokens")
+
+
+def _per_row(who: str, name: str, t, B: int, T: int, per_sequence: bool = False):
+    """(tensor, strides) of an fp32 input with one value per row: (B, T), or -- per_sequence -- (B,) / (B, 1) as well"""
+    if t is None:
+        return None, 0, 0
+    if t.dtype != torch.float32:
+        raise ValueError(f"{who}: {name} of type {t.dtype} (float32)")
+    if t.shape == (B, T):
+        return t, t.stride(0), t.stride(1)
+    if per_sequence and t.shape in ((B,), (B, 1)):
+        return t, t.stride(0), 0
+    raise ValueError(f"{who}: {name} of shape {tuple(t.shape)} for {B} sequences of {T} rows")
+
+
+def _row_args(logits, ids, mask, pad_idx):
+    B, T, V = logits.shape
+    mb, mt = (0, 0) if mask is None else mask.stride()
+    return (logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), logits.stride(1), B, T, V, ids.data_ptr(), ids.stride(0), ids.stride(1),
+            None if mask is None else mask.data_ptr(), mb, mt, _NO_PAD if pad_idx is None else int(pad_idx))
+
+
+def _logit_grad_buffer(logits):
+    """an empty gradient whose rows lie as the logits' rows do (same strides, same alignment: 16-byte stores wherever there were 16-byte loads),
+    or a contiguous one if those overlap or leave more room between them than they hold"""
+    if logits.is_contiguous() and logits.data_ptr() % 16 == 0:
+        return torch.empty_like(logits)
+    B, T, V = logits.shape
+    sb, st = logits.stride(0), logits.stride(1)
+    lo, hi = sorted(((sb, B), (st, T))) if B > 1 and T > 1 else ((0, 1), (sb, B) if B > 1 else (st, T))
+    apart = (lo[1] == 1 or lo[0] >= V) and (hi[1] == 1 or hi[0] >= lo[0] * (lo[1] - 1) + V)
+    span = (B - 1) * sb * (B > 1) + (T - 1) * st * (T > 1) + V
+    if not apart or span > 2 * B * T * V:
+        return torch.empty(B, T, V, device=logits.device, dtype=logits.dtype)
+    phase = logits.data_ptr() % 16 // logits.element_size()
+    buf = torch.empty(span + phase, device=logits.device, dtype=logits.dtype)
+    return buf.as_strided(logits.shape, (sb if B > 1 else T * V, st if T > 1 else V, 1), phase)
+
+
+def _last_dim_dense(logits):
+    return logits if logits.stride(2) == 1 or logits.shape[2] == 1 else logits.contiguous()
+
+
+def _logit_grad(logits, ids, mask, pad_idx, stats_ptr, w_ptr, wb, wt, g, out=None):
+    """d loss / d logits from a row's statistics and weight; ``out`` (bmt_policy_loss filled it): done unless the upstream gradient is not 1"""
+    once = out is not None
+    if out is None:
+        out = _logit_grad_buffer(logits)
+    if g is not None and g.dtype != torch.float32:
+        g = g.float()
+    _run_on(logits.device, "bmt_logit_grad", lib.bmt_logit_grad, *_row_args(logits, ids, mask, pad_idx), stats_ptr, w_ptr, wb, wt,
+            None if g is None else g.data_ptr(), int(once), out.data_ptr(), out.stride(0), out.stride(1))
+    return out
+
+
+class TokenLogpFn(torch.autograd.Function):
+    """log_softmax(logits)[ids], per row; the backward recomputes the softmax from the row's maximum and sum"""
+
+    @staticmethod
+    def forward(ctx, logits, ids, mask, pad_idx):
+        x = _last_dim_dense(logits)
+        B, T, _ = x.shape
+        logp = torch.empty(B, T, device=x.device, dtype=torch.float32)
+        stats = torch.empty(B, T, 2, device=x.device, dtype=torch.float32) if ctx.needs_input_grad[0] else None
+        _run_on(x.device, "bmt_logp_rows", lib.bmt_logp_rows, *_row_args(x, ids, mask, pad_idx), logp.data_ptr(), None if stats is None else stats.data_ptr())
+        ctx.save_for_backward(x, ids, mask, stats)
+        ctx.pad_idx = pad_idx
+        return logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d):
+        x, ids, mask, stats = ctx.saved_tensors
+        return _logit_grad(x, ids, mask, ctx.pad_idx, stats.data_ptr(), d.data_ptr(), d.stride(0), d.stride(1), None), None, None, None
+
+
+def token_logp(logits, ids, mask=None, pad_idx: Optional[int] = None):
+    """log-probabilities (B, T) fp32 of the tokens ``ids`` (B, T) under ``logits`` (B, T, V) of any float type and row strides -- or under a
+    Generator's log-probabilities: log-softmax leaves those as they are.  Rows that ``mask`` or ``pad_idx`` leave out are 0, are not read, and get
+    no gradient.  What a policy or preference loss takes as old and reference values."""
+    _check_rows("token_logp", logits, ids, mask)
+    _tuning_device("token_logp", logits, ids, mask)
+    return TokenLogpFn.apply(logits, ids, mask, pad_idx)
+
+
+class PolicyStats:
+    """what policy_loss saw: ``logp`` (B, T) of the tokens (0 where a row does not count), and the means over the rows that count of the KL term
+    (0 without a reference) and of the rows whose gradient the clip took -- device values, no graph"""
+    __slots__ = ("logp", "_info")
+
+    def __init__(self, logp, info):
+        self.logp, self._info = logp, info
+
+    @property
+    def kl(self):
+        return self._info[0]
+
+    @property
+    def clip_fraction(self):
+        return self._info[1]
+
+
+_REDUCTIONS = {"sum": 0, "token": 1, "sequence": 2}
+
+
+class PolicyLossFn(torch.autograd.Function):
+    """policy_loss: the forward leaves the logits' gradient for an upstream gradient of 1, so that every logit is read once; the backward launches
+    a kernel that ends at once if the upstream gradient IS 1 and computes the gradient again, from the logits, if not"""
+
+    @staticmethod
+    def forward(ctx, logits, ids, old, adv, ref, mask, pad_idx, lo, hi, beta, reduction):
+        x = _last_dim_dense(logits)
+        B, T, V = x.shape
+        dev = x.device
+        loss = torch.empty((), device=dev, dtype=torch.float32)
+        info = torch.empty(2, device=dev, dtype=torch.float32)
+        logp = torch.empty(B, T, device=dev, dtype=torch.float32)
+        n = lib.bmt_policy_ws_bytes(B, T)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8)
+        d = _logit_grad_buffer(x) if ctx.needs_input_grad[0] else None
+        db, dt = (0, 0) if d is None else (d.stride(0), d.stride(1))
+        old, ob, ot = _per_row("policy_loss", "old_logp", old, B, T)
+        ref, rb, rt = _per_row("policy_loss", "ref_logp", ref, B, T)
+        adv, ab, at = _per_row("policy_loss", "advantages", adv, B, T, per_sequence=True)
+        _run_on(dev, "bmt_policy_loss", lib.bmt_policy_loss, *_row_args(x, ids, mask, pad_idx), None if old is None else old.data_ptr(), ob, ot,
+                None if ref is None else ref.data_ptr(), rb, rt, adv.data_ptr(), ab, at, lo, hi, beta, reduction, loss.data_ptr(), info.data_ptr(),
+                logp.data_ptr(), ws.data_ptr(), n, None if d is None else d.data_ptr(), db, dt)
+        if d is not None:
+            ctx.save_for_backward(x, ids, mask, ws)
+            ctx.pad_idx, ctx.dlogits = pad_idx, d
+        ctx.mark_non_differentiable(info, logp)
+        ctx.set_materialize_grads(False)
+        return loss, info, logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _info, _logp):
+        if g is None:
+            return (None,) * 11
+        x, ids, mask, ws = ctx.saved_tensors
+        rows = x.shape[0] * x.shape[1]
+        out, ctx.dlogits = ctx.dlogits, None      # (a second backward pass through a kept graph computes its own)
+        d = _logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr() + 24 * rows, ws.data_ptr() + 32 * rows, x.shape[1], 1, g, out)
+        return (d,) + (None,) * 10
+
+
+def policy_loss(logits, ids, old_logp, advantages, ref_logp=None, mask=None, pad_idx: Optional[int] = None, clip_low: float = 0.2,
+                clip_high: float = 0.2, kl_coef: float = 0.0, reduction: str = "token"):
+    """Clipped policy loss of sampled tokens with a KL term, from logits (B, T, V) of any float type:
+        rho = exp(logp - old_logp),  -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1),  d = ref_logp - logp
+    over the rows that ``mask`` and ``pad_idx`` leave in; ``advantages`` (B,), (B, 1) or (B, T); ``old_logp`` None: the samples are the current
+    policy's own (rho = 1); ``reduction`` "token" (mean over those rows), "sequence" (mean over the sequences of their means) or "sum".  Returns
+    (loss, PolicyStats).  Only ``logits`` gets a gradient; while it wants one, the gradient is held from the forward pass on, and one backward
+    pass of ``loss`` itself (upstream gradient 1) costs no further read of the logits -- scale by ``reduction`` rather than afterwards."""
+    _check_rows("policy_loss", logits, ids, mask)
+    _tuning_device("policy_loss", logits, ids, mask, old_logp, advantages, ref_logp)
+    if ids.numel() == 0:
+        raise ValueError("policy_loss: no rows")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"policy_loss: reduction {reduction!r} (one of {sorted(_REDUCTIONS)})")
+    if not (clip_low >= 0 and clip_high >= 0):
+        raise ValueError(f"policy_loss: clip range ({clip_low}, {clip_high})")
+    if advantages is None:
+        raise ValueError("policy_loss: advantages are needed")
+    loss, info, logp = PolicyLossFn.apply(logits, ids, old_logp, advantages, ref_logp, mask, pad_idx, float(clip_low), float(clip_high), float(kl_coef),
+                                          _REDUCTIONS[reduction])
+    return loss, PolicyStats(logp, info)
+
+
+class PreferenceLossFn(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, logits, ids, ref, mask, pad_idx, beta, smoothing, mean):
+        x = _last_dim_dense(logits)
+        B, T, V = x.shape
+        dev = x.device
+        loss = torch.empty((), device=dev, dtype=torch.float32)
+        rewards = torch.empty(B, device=dev, dtype=torch.float32)
+        n = lib.bmt_preference_ws_bytes(B, T)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8)
+        _run_on(dev, "bmt_preference_loss", lib.bmt_preference_loss, *_row_args(x, ids, mask, pad_idx), ref.data_ptr(), ref.stride(0), beta, smoothing,
+                int(mean), loss.data_ptr(), rewards.data_ptr(), ws.data_ptr(), n)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(x, ids, mask, ws)
+            ctx.pad_idx = pad_idx
+        ctx.mark_non_differentiable(rewards)
+        ctx.set_materialize_grads(False)
+        return loss, rewards
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _rewards):
+        if g is None:
+            return (None,) * 8
+        x, ids, mask, ws = ctx.saved_tensors
+        rows = x.shape[0] * x.shape[1]
+        return (_logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr(), ws.data_ptr() + 8 * rows, 1, 0, g),) + (None,) * 7
+
+
+def preference_loss(logits, ids, ref_logp, mask=None, pad_idx: Optional[int] = None, beta: float = 0.1, label_smoothing: float = 0.0,
+                    mean_logp: bool = False):
+    """Paired preference loss from logits (B, T, V) of any float type: sequence b < B / 2 is preferred to sequence b + B / 2.
+        S_b = sum (mean_logp: mean) of the log-probabilities of the rows that ``mask`` and ``pad_idx`` leave in,  r_b = beta (S_b - ref_logp[b]),
+        loss = mean over pairs of -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z),  z = r_b - r_{b + B / 2}
+    ``ref_logp`` (B,): S_b under the reference model.  Returns (loss, rewards (B,)); only ``logits`` gets a gradient."""
+    _check_rows("preference_loss", logits, ids, mask)
+    _tuning_device("preference_loss", logits, ids, mask, ref_logp)
+    B = logits.shape[0]
+    if B == 0 or B % 2 or ids.numel() == 0:
+        raise ValueError(f"preference_loss: {B} sequences of {ids.shape[1]} tokens are not pairs")
+    if ref_logp.shape != (B,) or ref_logp.dtype != torch.float32:
+        raise ValueError(f"preference_loss: ref_logp of shape {tuple(ref_logp.shape)} and type {ref_logp.dtype} (float32 ({B},))")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"preference_loss: label_smoothing {label_smoothing}")
+    return PreferenceLossFn.apply(logits, ids, ref_logp, mask, pad_idx, float(beta), float(label_smoothing), bool(mean_logp))
+
+
+def _embedding_forward(idc, W, scale):
+    V, D = W.shape
+    out = torch.empty(*idc.shape, D, device=W.device, dtype=W.dtype)
+    _run_on(W.device, "bmt_embedding", lib.bmt_embedding, idc.data_ptr(), W.data_ptr(), W.stride(0), out.data_ptr(), idc.numel(), D, V, _DTYPES[W.dtype], scale)
+    return out
+
+
+class EmbeddingFn(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, ids, W, scale, pad_idx):
+        ctx.save_for_backward(ids)
+        ctx.meta = (W.shape, scale, pad_idx)
+        ctx.weight = W
+        note_use(W)
+        return _embedding_forward(ids, W, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        (V, D), scale, pad_idx = ctx.meta
+        n = ids.numel()
+        d2 = dy.reshape(n, D)
+        if D > 1 and d2.stride(1) != 1:
+            d2 = d2.contiguous()
+        gW = static_grad(ctx.weight)
+        if gW is not None and (gW.shape != (V, D) or gW.dtype != torch.float32 or d2.dtype != torch.float32):
+            gW = None
+        dW = torch.empty(V, D, device=dy.device, dtype=dy.dtype) if gW is None else None
+        nws = lib.bmt_embedding_bwd_ws_bytes(n, D, V)
+        ws = torch.empty(nws, device=dy.device, dtype=torch.uint8)
+        _run_on(dy.device, "bmt_embedding_bwd", lib.bmt_embedding_bwd, ids.data_ptr(), d2.data_ptr(), d2.stride(0), n, D, V, _DTYPES[dy.dtype], scale,
+                _NO_PAD if pad_idx is None else int(pad_idx), None if dW is None else dW.data_ptr(), None if gW is None else gW.data_ptr(), D, ws.data_ptr(), nws)
+        if gW is not None:
+            grad_done(ctx.weight)
+        return None, dW, None, None
+
+
+def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
+    """scale * weight[ids] (ids int64 of any shape; weight (V, D) fp32, bf16 or fp16; ids outside the table are clamped, as EmbedFn does).  The
+    gradient of ``weight`` is added in fp32 over a token's positions in ascending order and rounded once -- the same bits on every run, whichever
+    tokens repeat --; ``pad_idx`` gets none.  A parameter with a static gradient buffer (GradientReducer) has it added there directly."""
+    _tuning_device("embedding", ids, weight)
+    if weight.dim() != 2 or weight.dtype not in _DTYPES or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"embedding: a weight of shape {tuple(weight.shape)} and type {weight.dtype} (2-D float32, bfloat16 or float16)")
+    if ids.dtype != torch.int64:
+        raise ValueError(f"embedding: ids of type {ids.dtype} (int64)")
+    if ids.numel() > 0x7fffffff - 64:
+        raise ValueError(f"embedding: {ids.numel()} ids")
+    if weight.stride(0) < weight.shape[1] or (weight.shape[1] > 1 and weight.stride(1) != 1):
+        weight = weight.contiguous()
+    idc = ids.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return EmbeddingFn.apply(idc, weight, float(scale), pad_idx)
+    return _embedding_forward(idc, weight, float(scale))

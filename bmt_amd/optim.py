@@ -6,12 +6,13 @@ launch over every parameter.  Subclasses torch.optim.Optimizer so ``state_dict()
 (``exp_avg`` / ``exp_avg_sq`` / ``step`` per parameter) and checkpoints interchange."""
 from __future__ import annotations
 
-from typing import Iterable, List
+from typing import Iterable, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import _lib
-from .ops import _p, _st, lib
+from .ops import _DTYPES, _p, _run_on, _st, lib
 
 
 class _PtrTable:
@@ -135,3 +136,107 @@ def clip_grad_norm_(parameters: Iterable[torch.nn.Parameter], max_norm: float) -
                "bmt_grad_sqnorm")
     _lib.check(lib.bmt_scale_tensors(_p(tab.ptrs), _p(tab.sizes), tab.n, tab.max_size, _p(coef), _st()), "bmt_scale_tensors")
     return sq.sqrt().squeeze(0)
+
+
+CLIP_TILE = 8192        # elements per tile of GradClipper's table: 32 per thread of a workgroup
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """whether the elements fill a range of memory, in any order of the dimensions"""
+    n = 1
+    if t.numel() == 0:
+        return True
+    for size, stride in sorted(((a, b) for a, b in zip(t.shape, t.stride()) if a != 1), key=lambda x: x[1]):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+class GradClipper:
+    """Global norm of many gradient tensors, and clipping -- ``clip_grad_norm_`` for gradients of mixed types, for a captured step and for
+    buffers other than the gradients' own:
+
+        clipper = GradClipper([p.grad for p in params], max_norm=1.0)      # static gradient buffers (GradientReducer keeps such)
+        total = clipper()                                                  # norm as a device scalar; gradients *= min(1, max_norm / (norm + eps))
+
+    ``grads``: fp32, bf16 or fp16 tensors on one device, dense in any order of their dimensions, none sharing memory with another.  ``out``: one
+    tensor per gradient (same shape and order of dimensions, its own type) that takes the clipped values -- what FusedAdam wants of 16-bit
+    gradients --; None: in place.  ``norm_type``: 2 or inf.  ``clipper(scale=s)``: s (device float) is a factor the gradients still lack: norm and
+    result are those of s * gradient.  ``clipper(apply=False)``: the norm alone.  ``clipper.coef``: the last call's factor min(1, ..) * s, for
+    FusedAdam.grad_scale.  A non-finite norm does what it does in torch: inf leaves finite gradients 0, NaN makes them NaN.
+
+    Sums are 64-bit and in one order: the same bits on every run.  The plan holds the tensors, and a call refuses ones whose memory has moved."""
+
+    def __init__(self, grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None, norm_type: float = 2.0, eps: float = 1e-6):
+        self.grads = list(grads)
+        self.out = self.grads if out is None else list(out)
+        self.max_norm, self.eps = float(max_norm), float(eps)
+        if not self.grads:
+            raise ValueError("GradClipper: no gradients")
+        if norm_type not in (2, float("inf")):
+            raise ValueError(f"GradClipper: norm_type {norm_type} (2 or inf)")
+        self._inf = int(norm_type != 2)
+        if not (self.max_norm >= 0.0 and self.eps >= 0.0):
+            raise ValueError(f"GradClipper: max_norm {max_norm}, eps {eps}")
+        if len(self.out) != len(self.grads):
+            raise ValueError(f"GradClipper: {len(self.out)} output tensors for {len(self.grads)} gradients")
+        for t in self.grads + ([] if out is None else self.out):
+            if not t.is_cuda:
+                raise RuntimeError("GradClipper: bmt_amd ops need CUDA/HIP tensors: there is no CPU fallback")
+            if t.device != self.grads[0].device or t.dtype not in _DTYPES or not _dense(t):
+                raise ValueError(f"GradClipper: a tensor of shape {tuple(t.shape)}, strides {t.stride()} and type {t.dtype} on {t.device}: all are dense, "
+                                 "float32, bfloat16 or float16, and on one device")
+        for g, o in zip(self.grads, self.out):
+            if g.shape != o.shape or any(a != 1 and g.numel() > 0 and x != y for a, x, y in zip(g.shape, g.stride(), o.stride())):
+                raise ValueError(f"GradClipper: a gradient of shape {tuple(g.shape)} and strides {g.stride()} with an output of {tuple(o.shape)} and {o.stride()}")
+        self.device = self.grads[0].device
+        self._ptrs = [t.data_ptr() for t in self.grads], [t.data_ptr() for t in self.out]
+        self._in_place = int(all(g.dtype == o.dtype for g, o in zip(self.grads, self.out)) and self._ptrs[0] == self._ptrs[1])
+        self._refuse_shared_memory()
+        self.coef = None
+        self._tiles, self._n = self._table()
+
+    def _refuse_shared_memory(self):
+        ranges = []
+        for g, o, pg, po in zip(self.grads, self.out, *self._ptrs):
+            if g.numel() == 0:
+                continue
+            ranges.append((pg, pg + g.numel() * g.element_size()))
+            if po != pg or o.dtype != g.dtype:
+                ranges.append((po, po + o.numel() * o.element_size()))
+        ranges.sort()
+        if any(a[1] > b[0] for a, b in zip(ranges, ranges[1:])):
+            raise ValueError("GradClipper: two of the tensors share memory (a gradient given twice, or an output that overlaps another tensor)")
+
+    def _table(self):
+        entry = np.dtype([("g", "<u8"), ("out", "<u8"), ("n", "<i4"), ("kind", "<i4")])
+        assert entry.itemsize == lib.bmt_clip_tile_bytes()
+        rows = []
+        for g, o, pg, po in zip(self.grads, self.out, *self._ptrs):
+            first = np.arange(0, g.numel(), CLIP_TILE, dtype=np.uint64)
+            r = np.empty(len(first), entry)
+            r["g"], r["out"] = pg + first * np.uint64(g.element_size()), po + first * np.uint64(o.element_size())
+            r["n"] = np.minimum(CLIP_TILE, g.numel() - first.astype(np.int64))
+            r["kind"] = _DTYPES[g.dtype] | _DTYPES[o.dtype] << 2
+            rows.append(r)
+        rows = np.concatenate(rows)
+        if len(rows) > 0x7fffffff:
+            raise ValueError("GradClipper: too many elements")
+        return torch.from_numpy(rows.view(np.uint8)).to(self.device), len(rows)
+
+    @torch.no_grad()
+    def __call__(self, scale: Optional[torch.Tensor] = None, apply: bool = True) -> torch.Tensor:
+        if ([t.data_ptr() for t in self.grads], [t.data_ptr() for t in self.out]) != self._ptrs:
+            raise RuntimeError("GradClipper: a tensor's memory has moved since the plan was made: make a new one")
+        if scale is not None and (scale.numel() != 1 or scale.dtype != torch.float32 or scale.device != self.device):
+            raise ValueError(f"GradClipper: scale is one float32 value on {self.device}")
+        result = torch.empty(2, device=self.device, dtype=torch.float32)
+        n = lib.bmt_clip_ws_bytes()
+        ws = torch.empty(n, device=self.device, dtype=torch.uint8)      # (of this call: two captured graphs, or two streams, share nothing)
+        _run_on(self.device, "bmt_clip_grads", lib.bmt_clip_grads, self._tiles.data_ptr() if self._n else None, self._n, self._inf, self.max_norm, self.eps,
+                None if scale is None else scale.data_ptr(), int(apply), self._in_place, result.data_ptr(), ws.data_ptr(), n)
+        if apply:
+            torch.autograd.graph.increment_version(self.out)
+        self.coef = result[1]
+        return result[0]

@@ -621,6 +621,63 @@ int bmt_caption_shift(const int64_t* caption_idx, int64_t ld, int B, int T1, int
 /* loss[0] = kl[0] / n_tokens[0], grad_scale[0] = 1 / n_tokens[0] (either output may be NULL): loss = criterion(pred, y) / n_tokens */
 int bmt_loss_finish(const float* kl, const int64_t* n_tokens, float* loss, float* grad_scale, void* stream);
 
+/* ---------------------------------------------------------------- tuning a caption model: losses on sampled tokens, embedding, gradient norm
+ * Element types of the operators below (tensors that are not fp32 throughout). */
+#define BMT_DT_F32 0
+#define BMT_DT_BF16 1
+#define BMT_DT_F16 2
+/* Rows (b, t), b < B, t < T: logits + b * sb + t * st (V contiguous elements of `dtype`, aligned to their size; any strides >= 0, also
+ * overlapping ones), ids + b * ib + t * it (int64), mask + b * mb + t * mt (uint8, NULL = all 1).  A row COUNTS iff its mask is non-zero and its
+ * id is not pad_idx (INT64_MIN: no padding id); a row that does not count is not read, its log-probability is 0 and its gradient row is zeros.
+ * An id outside [0, V) in a row that counts gives NaN.
+ *   bmt_logp_rows        logp[b * T + t] = log softmax(row)[id]; stats (optional, [B * T][2]): maximum and 1 / sum for bmt_logit_grad
+ *   bmt_logit_grad       dlogits row = g w (1[c = id] - softmax(row)), w at b * wb + t * wt, g = *gscale_dev (NULL = 1), written at
+ *                        dlogits + b * db + t * dt in `dtype`.  once != 0: dlogits already holds the gradient for g = 1 (bmt_policy_loss), and
+ *                        nothing is read or written if g is 1
+ *   bmt_policy_loss      rho = exp(logp - old), row loss -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1) with
+ *                        d = ref - logp; old_logp NULL: rho = 1 (its gradient stays that of rho), ref_logp NULL: no KL term.  reduction 0: sum,
+ *                        1: mean over the rows that count, 2: mean over the B sequences of their means (0 where nothing counts).
+ *                        loss[0]; info[0] = mean KL, info[1] = share of rows whose policy gradient the clip took; logp [B * T].  dlogits
+ *                        (optional): the gradient of loss, in the same pass.  ws: bmt_policy_ws_bytes, 8-byte aligned; it keeps what
+ *                        bmt_logit_grad wants: stats at 24 * B * T bytes, w (wb = T, wt = 1) at 32 * B * T bytes
+ *   bmt_preference_loss  sequences b and b + B / 2 are a pair (preferred, rejected): S_b = sum of logp over the rows that count (mean_logp: their
+ *                        mean), rewards[b] = beta (S_b - ref_logp[b * ref_stride]), loss[0] = mean of -(1 - smoothing) log sigmoid(z) -
+ *                        smoothing log sigmoid(-z), z = the difference of a pair's rewards.  ws: bmt_preference_ws_bytes, 8-byte aligned; stats at
+ *                        0, w (wb = 1, wt = 0) at 8 * B * T bytes */
+int bmt_logp_rows(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
+                  const uint8_t* mask, int64_t mb, int64_t mt, int64_t pad_idx, float* logp, float* stats, void* stream);
+int bmt_logit_grad(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
+                   const uint8_t* mask, int64_t mb, int64_t mt, int64_t pad_idx, const float* stats, const float* w, int64_t wb, int64_t wt,
+                   const float* gscale_dev, int once, void* dlogits, int64_t db, int64_t dt, void* stream);
+int64_t bmt_policy_ws_bytes(int B, int T);
+int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
+                    const uint8_t* mask, int64_t mb, int64_t mt, int64_t pad_idx, const float* old_logp, int64_t ob, int64_t ot,
+                    const float* ref_logp, int64_t rb, int64_t rt, const float* adv, int64_t ab, int64_t at, float clip_low, float clip_high,
+                    float kl_coef, int reduction, float* loss, float* info, float* logp, void* ws, int64_t ws_bytes, void* dlogits, int64_t db,
+                    int64_t dt, void* stream);
+int64_t bmt_preference_ws_bytes(int B, int T);
+int bmt_preference_loss(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
+                        const uint8_t* mask, int64_t mb, int64_t mt, int64_t pad_idx, const float* ref_logp, int64_t ref_stride, float beta,
+                        float smoothing, int mean_logp, float* loss, float* rewards, void* ws, int64_t ws_bytes, void* stream);
+/* out[n][0 .. D) = scale * W[ids[n]][0 .. D) (W rows at stride ldw, out contiguous, both `dtype`); ids outside [0, V) are clamped as in
+ * bmt_prep_embed */
+int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, void* out, int64_t N, int D, int V, int dtype, float scale, void* stream);
+/* its gradient, the same bits on every run: row v = scale * sum of dout[n] over the positions n with ids[n] == v, added in fp32 in ascending
+ * order of n; positions that hold pad_idx are left out (INT64_MIN: none).  dW ([V][D] at stride ldw, `dtype`): every row is written, zeros
+ * where a token does not occur -- or into (fp32): the rows of the tokens that occur are added to it.  ws: bmt_embedding_bwd_ws_bytes, 16-byte
+ * aligned */
+int64_t bmt_embedding_bwd_ws_bytes(int64_t N, int D, int V);
+int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t ld, int64_t N, int D, int V, int dtype, float scale, int64_t pad_idx, void* dW,
+                      float* into, int64_t ldw, void* ws, int64_t ws_bytes, void* stream);
+/* Global norm of many tensors and clipping.  tiles: DEVICE table of n_tiles entries of bmt_clip_tile_bytes() = 24 bytes {const void* g; void*
+ * out; int32 n; int32 kind = dtype of g | dtype of out << 2}: n elements each.  norm = |s| sqrt(sum g^2) (norm_inf: |s| max |g|), s =
+ * *scale_dev (NULL = 1); c = s * min(1, max_norm / (norm + eps)); result[0] = norm, result[1] = c; apply: out = c g for every tile, in_place
+ * (every out is its g): nothing is touched if c is 1.  ws: bmt_clip_ws_bytes, 8-byte aligned.  Sums in 64 bits, in one order. */
+int bmt_clip_tile_bytes(void);
+int64_t bmt_clip_ws_bytes(void);
+int bmt_clip_grads(const void* tiles, int n_tiles, int norm_inf, float max_norm, float eps, const float* scale_dev, int apply, int in_place,
+                   float* result, void* ws, int64_t ws_bytes, void* stream);
+
 /* ---------------------------------------------------------------- optimizer (K11) */
 /* torch.optim.Adam semantics (scripts/train_captioning_module.py:46-48) over n_tensors tensors.
  * ptrs: device array of 4*n_tensors pointers laid out [p_0..][g_0..][m_0..][v_0..]; sizes: device int64[n].
