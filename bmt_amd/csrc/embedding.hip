@@ -2,8 +2,10 @@
 //   out[n] = scale W[id_n]                              dW[v] = scale sum_{n : id_n = v} dout[n]
 // Bound: HBM -- the lookup reads N rows and writes N rows, the gradient reads N rows and writes V rows, one or two operations per element.
 // The gradient sums in fp32 over the positions of a token in ascending order, rounded once: no atomics, the same bits on every run.  Three launches:
-//   order  every workgroup owns a range of the vocabulary, reads ALL ids (they come from L2: 8 bytes against a row of hundreds) and places the
-//          positions of its tokens, in order, behind the count of the tokens below its range -- no second pass over a global histogram
+//   order  workgroup g of G owns the tokens v = g (mod G) -- frequent tokens are neighbours in most vocabularies, and contiguous ranges would give
+//          one workgroup half of a text --, reads ALL ids (they come from L2: 8 bytes against a row of hundreds) and places the positions of its
+//          tokens, in order, behind the count of the tokens of lower owners: no second pass over a global histogram.  Many ids are split by owner
+//          first (two small launches, the same counting by owner instead of by token): G readers of all ids cost 57 us for 65536
 //   sum    a wave per (token, block of columns) adds a token's rows if they are at most EMB_LONG; the rows of more frequent tokens are added
 //          EMB_LONG sorted positions at a time by workgroups of their own (a few tokens hold half of a text)
 //   join   adds those partial sums per token, in order
@@ -12,7 +14,22 @@
 namespace {
 
 constexpr int EMB_LONG = 32;        // positions a wave adds by itself; also the sorted positions per partial sum: a longer run starts in at most one of them
+constexpr int EMB_FEW = 2048;       // up to here a frequent token's rows are added by the workgroup that meets it (a launch less), beyond by many
+constexpr int EMB_DIRECT = 8192;    // up to here every owner reads all ids; beyond, the ids are split by owner first
+constexpr int EMB_SPLIT_G = 512;    // most owners the split is made for (its LDS: 16 waves x owners)
 constexpr int EMB_BINS = 960;       // most tokens a workgroup of the order kernel owns: one per thread in its scan, 60 KB of LDS
+
+// the sorted order's index of a token: owner v mod G first, then v / G (G = 1 << lg owners of nb tokens each)
+struct Owners {
+    int lg, nb;
+    __device__ __forceinline__ int slot(int v) const { return (v & ((1 << lg) - 1)) * nb + (v >> lg); }
+    __device__ __forceinline__ int token(int u) const { return ((u % nb) << lg) + u / nb; }
+};
+
+// ids split by owner: those of owner g stand at start[g] .. start[g + 1), as positions and numbers v / G
+struct Split {
+    int *start, *pos, *key;
+};
 
 __device__ __forceinline__ int clamp_id(int64_t id, int V) { return id < 0 ? 0 : (id >= V ? V - 1 : (int)id); }
 
@@ -93,30 +110,35 @@ __global__ __launch_bounds__(256) void embed_kernel(const int64_t* __restrict__ 
         }
 }
 
-// ---------------------------------------------------------------- order: stable counting sort, a range of tokens per workgroup
+// ---------------------------------------------------------------- order: stable counting sort, an owner's tokens per workgroup
 // Wave w walks the ids [w * chunk, (w + 1) * chunk); K > 0: a lane keeps its K ids in registers between counting and placing (N <= 1024 K),
-// K = 0: they are read twice.  offsets[v] = first sorted position of token v, offsets[V] = the positions that count (the padding id does not).
+// K = 0: they are read twice; K = -1: the owner's ids were split off (sp).  offsets[u] = first sorted position of the token in slot u, offsets[slots] = the positions that count (the padding
+// id does not).  Placing 64 positions: the lanes that hold one token find each other by a ballot per bit of its number -- the cost does not depend
+// on how many different tokens they hold (one round per different token took 245 us for 65536 Zipf-distributed ids, 10 times as long).
 template <int K>
-__global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __restrict__ ids, int64_t N, int V, int64_t pad, int nb, int* __restrict__ offsets,
-                                                            int* __restrict__ order, int* __restrict__ token) {
+__global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __restrict__ ids, int64_t N, int V, int64_t pad, Owners ow, int bits, int slots, Split sp,
+                                                            int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ slot) {
     extern __shared__ int hist[];      // [16][nb]
     __shared__ int wsum[16], wbelow[16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int v0 = blockIdx.x * nb, nv = min(nb, V - v0);
+    const int nb = ow.nb, me = blockIdx.x, gmask = (1 << ow.lg) - 1;
     for (int i = threadIdx.x; i < 16 * nb; i += 1024) hist[i] = 0;
     __syncthreads();
-    const int64_t chunk = ((N + 15) / 16 + 63) / 64 * 64, first = wave * chunk, last = min(N, first + chunk);
+    const int64_t from = K < 0 ? sp.start[me] : 0, until = K < 0 ? sp.start[me + 1] : N;
+    const int64_t chunk = ((until - from + 15) / 16 + 63) / 64 * 64, first = from + wave * chunk, last = min(until, first + chunk);
     int* mine = hist + wave * nb;
-    int key[K > 0 ? K : 1];      // the token relative to the range; below it: negative; the padding id and positions behind the end: INT_MAX
-    int below = 0;
+    int key[K > 0 ? K : 1];      // a token of this owner: its number v / G; of a lower owner: -1; else (and the padding id, and behind the end): -2
+    int below = K < 0 && threadIdx.x == 0 ? (int)from : 0;
     auto fetch = [&](int64_t n) -> int {
-        if (n >= last) return 0x7fffffff;
+        if (n >= last) return -2;
+        if constexpr (K < 0) return sp.key[n];
         const int64_t id = ids[n];
-        return id == pad ? 0x7fffffff : clamp_id(id, V) - v0;
+        const int v = clamp_id(id, V), o = v & gmask;
+        return id == pad || o > me ? -2 : (o < me ? -1 : v >> ow.lg);
     };
     auto count = [&](int k) {
-        if (k < 0) ++below;
-        else if (k < nv) atomicAdd(&mine[k], 1);
+        if (k == -1) ++below;
+        else if (k >= 0) atomicAdd(&mine[k], 1);
     };
     if constexpr (K > 0) {
 #pragma unroll
@@ -138,7 +160,7 @@ __global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __rest
     __syncthreads();
     // exclusive scan of the tokens' totals (one token per thread), then of each token's counts over the waves
     int total = 0;
-    if ((int)threadIdx.x < nv)
+    if ((int)threadIdx.x < nb)
         for (int w = 0; w < 16; ++w) total += hist[w * nb + threadIdx.x];
     int scan = total;
 #pragma unroll
@@ -153,9 +175,10 @@ __global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __rest
         start += wbelow[w];
         if (w < wave) start += wsum[w];
     }
-    if ((int)threadIdx.x < nv) {
-        offsets[v0 + threadIdx.x] = start;
-        if (v0 + (int)threadIdx.x == V - 1) offsets[V] = start + total;
+    if ((int)threadIdx.x < nb) {
+        const int u = me * nb + threadIdx.x;
+        offsets[u] = start;
+        if (u == slots - 1) offsets[slots] = start + total;
         for (int w = 0, at = start; w < 16; ++w) {
             const int h = hist[w * nb + threadIdx.x];
             hist[w * nb + threadIdx.x] = at;
@@ -163,28 +186,120 @@ __global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __rest
         }
     }
     __syncthreads();
-    auto place = [&](int k, int64_t n) {      // 64 positions: the lanes of one token at a time, in lane order
-        const bool in = k >= 0 && k < nv;
-        uint64_t todo = __ballot(in);
-        while (todo) {
-            const int lead = __ffsll((unsigned long long)todo) - 1, kl = __shfl(k, lead, 64);
-            const uint64_t same = __ballot(in && k == kl);
-            int at = 0;
-            if (lane == lead) at = atomicAdd(&mine[kl], (int)__popcll(same));
-            at = __shfl(at, lead, 64);
-            if (in && k == kl) {
-                const int p = at + (int)__popcll(same & ((1ull << lane) - 1));
-                order[p] = (int)n;
-                token[p] = v0 + k;
-            }
-            todo &= ~same;
+    auto place = [&](int k, int64_t n) {
+        const bool in = k >= 0;
+        uint64_t same = __ballot(in);
+        if (!same) return;
+        for (int b = 0; b < bits; ++b) {
+            const bool one = (k >> b) & 1;
+            const uint64_t ones = __ballot(one);
+            same &= one ? ones : ~ones;
         }
+        if (!in) return;
+        const int rank = (int)__popcll(same & ((1ull << lane) - 1));
+        int at = 0;
+        if (rank == 0) at = atomicAdd(&mine[k], (int)__popcll(same));
+        at = __shfl(at, __ffsll((unsigned long long)same) - 1, 64) + rank;
+        order[at] = K < 0 ? sp.pos[n] : (int)n;
+        slot[at] = me * nb + k;
     };
     if constexpr (K > 0) {
 #pragma unroll
         for (int i = 0; i < K; ++i) place(key[i], first + i * 64 + lane);
     } else {
         for (int64_t n = first; n < last; n += 64) place(fetch(n + lane), n + lane);
+    }
+}
+
+// ids by owner, per chunk of 1024 R: counts[chunk][owner]
+__global__ __launch_bounds__(1024) void embed_count_kernel(const int64_t* __restrict__ ids, int64_t N, int V, int64_t pad, Owners ow, int R, int* __restrict__ counts) {
+    __shared__ int hist[EMB_SPLIT_G];
+    const int G = 1 << ow.lg;
+    for (int i = threadIdx.x; i < G; i += 1024) hist[i] = 0;
+    __syncthreads();
+    for (int i = 0; i < R; ++i) {
+        const int64_t n = ((int64_t)blockIdx.x * R + i) * 1024 + threadIdx.x;
+        if (n < N) {
+            const int64_t id = ids[n];
+            if (id != pad) atomicAdd(&hist[clamp_id(id, V) & (G - 1)], 1);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < G; i += 1024) counts[(int64_t)blockIdx.x * G + i] = hist[i];
+}
+
+// ... and their places: owner by owner, chunk by chunk, in order within a chunk (as embed_order_kernel places tokens).  Every workgroup adds up the
+// counts itself: G x chunks integers from L2
+__global__ __launch_bounds__(1024) void embed_split_kernel(const int64_t* __restrict__ ids, int64_t N, int V, int64_t pad, Owners ow, int R, const int* __restrict__ counts, Split sp) {
+    __shared__ int hist[16 * EMB_SPLIT_G], low[1024], all[1024], wsum[16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int G = 1 << ow.lg, chunks = gridDim.x, me = blockIdx.x, parts = 1024 / G, o = threadIdx.x & (G - 1), part = threadIdx.x >> ow.lg;
+    for (int i = threadIdx.x; i < 16 * G; i += 1024) hist[i] = 0;
+    int lo = 0, total = 0;      // the owner's ids in lower chunks and in all, as this thread's share of the chunks
+#pragma unroll 8
+    for (int c = part; c < chunks; c += parts) {
+        const int k = counts[(int64_t)c * G + o];
+        total += k;
+        lo += c < me ? k : 0;
+    }
+    low[threadIdx.x] = lo;
+    all[threadIdx.x] = total;
+    __syncthreads();
+    const int64_t first = ((int64_t)me * 16 + wave) * 64 * R;
+    int* mine = hist + wave * G;
+    auto fetch = [&](int64_t n) -> int {
+        if (n >= N) return -1;
+        const int64_t id = ids[n];
+        return id == pad ? -1 : clamp_id(id, V);
+    };
+    for (int i = 0; i < R; ++i) {
+        const int v = fetch(first + i * 64 + lane);
+        if (v >= 0) atomicAdd(&mine[v & (G - 1)], 1);
+    }
+    lo = total = 0;
+    if ((int)threadIdx.x < G)
+        for (int p = 0; p < parts; ++p) {
+            lo += low[p * G + threadIdx.x];
+            total += all[p * G + threadIdx.x];
+        }
+    int scan = total;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(scan, d, 64);
+        if (lane >= d) scan += up;
+    }
+    if (lane == 63) wsum[wave] = scan;
+    __syncthreads();
+    int start = scan - total;
+    for (int w = 0; w < wave; ++w) start += wsum[w];
+    if ((int)threadIdx.x < G) {
+        if (me == 0) {
+            sp.start[threadIdx.x] = start;
+            if ((int)threadIdx.x == G - 1) sp.start[G] = start + total;
+        }
+        for (int w = 0, at = start + lo; w < 16; ++w) {
+            const int h = hist[w * G + threadIdx.x];
+            hist[w * G + threadIdx.x] = at;
+            at += h;
+        }
+    }
+    __syncthreads();
+    for (int i = 0; i < R; ++i) {
+        const int64_t n = first + i * 64 + lane;
+        const int v = fetch(n), k = v & (G - 1);
+        uint64_t same = __ballot(v >= 0);
+        for (int b = 0; b < ow.lg; ++b) {
+            const bool one = (k >> b) & 1;
+            const uint64_t ones = __ballot(one);
+            same &= one ? ones : ~ones;
+        }
+        if (v < 0) continue;
+        const int rank = (int)__popcll(same & ((1ull << lane) - 1));
+        int at = 0;
+        if (rank == 0) at = atomicAdd(&mine[k], (int)__popcll(same));
+        at = __shfl(at, __ffsll((unsigned long long)same) - 1, 64) + rank;
+        sp.key[at] = v >> ow.lg;
+        sp.pos[at] = (int)n;
     }
 }
 
@@ -233,22 +348,22 @@ __device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, i
 // workgroups [0, chunks * ncb): partial sums of the frequent tokens; behind them: a wave per (token, block of columns)
 template <int DT, int G>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__ dout, int64_t ld, const int* __restrict__ offsets, const int* __restrict__ order,
-                                                         const int* __restrict__ token, float* __restrict__ part, int64_t ldp, char* __restrict__ dW,
-                                                         float* __restrict__ into, int64_t ldw, int D, int V, float scale, int chunks, int ncb) {
+                                                         const int* __restrict__ slot, float* __restrict__ part, int64_t ldp, char* __restrict__ dW,
+                                                         float* __restrict__ into, int64_t ldw, int D, int V, Owners ow, int slots, float scale, int chunks, int ncb) {
     __shared__ float red[3][64 * G];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t wg = blockIdx.x, nlong = (int64_t)chunks * ncb;
     if (wg < nlong) {
         const int k = (int)(wg / ncb), c = ((int)(wg % ncb) * 64 + lane) * G;
         const bool in = c < D;
-        const int p0 = k * EMB_LONG, p1 = min(p0 + EMB_LONG, offsets[V]);
+        const int p0 = k * EMB_LONG, p1 = min(p0 + EMB_LONG, offsets[slots]);
         if (p0 >= p1) return;
-        const int t0 = token[p0], t1 = token[p1 - 1];
+        const int t0 = slot[p0], t1 = slot[p1 - 1];
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {      // at most the run that reaches into the chunk and the run that reaches out of it are long
-            const int v = h ? t1 : t0;
+            const int u = h ? t1 : t0;
             if (h && t1 == t0) break;
-            const int a = offsets[v], b = offsets[v + 1];
+            const int a = offsets[u], b = offsets[u + 1];
             if (b - a <= EMB_LONG) continue;
             const int q0 = max(p0, a), q1 = min(p1, b), each = (q1 - q0 + 3) / 4;
             float acc[G] = {};
@@ -267,27 +382,53 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
         return;
     }
     const int64_t task = (wg - nlong) * 4 + wave;
-    if (task >= (int64_t)V * ncb) return;
-    const int v = (int)(task / ncb), c = ((int)(task % ncb) * 64 + lane) * G;
+    const bool have = task < (int64_t)V * ncb;
+    const int v = have ? (int)(task / ncb) : 0, c = ((int)(task % ncb) * 64 + lane) * G;
     const bool in = c < D;
-    const int a = offsets[v], b = offsets[v + 1];
-    if (b - a > EMB_LONG || (into && a == b)) return;
-    float acc[G] = {};
-    add_rows<DT, G>(dout, ld, order, a, b, c, in, acc);
-    if (in) finish_row<DT, G>(dW, into, ldw, v, c, scale, acc);
+    const int u = ow.slot(v), a = offsets[u], b = have ? offsets[u + 1] : a;
+    const bool rare = b - a <= EMB_LONG;
+    if (rare && have && !(into && a == b)) {
+        float acc[G] = {};
+        add_rows<DT, G>(dout, ld, order, a, b, c, in, acc);
+        if (in) finish_row<DT, G>(dW, into, ldw, v, c, scale, acc);
+    }
+    if (chunks) return;
+    // no partial sums: the four waves share each frequent token that one of them met
+    __shared__ int4 met[4];
+    if (lane == 0) met[wave] = make_int4(rare ? 0 : a, rare ? 0 : b, v, (int)(task % ncb));
+    __syncthreads();
+#pragma unroll 1
+    for (int t = 0; t < 4; ++t) {
+        const int4 m = met[t];
+        if (m.x == m.y) continue;
+        const int mc = (m.w * 64 + lane) * G, each = (m.y - m.x + 3) / 4;
+        const bool inside = mc < D;
+        float acc[G] = {};
+        add_rows<DT, G>(dout, ld, order, min(m.y, m.x + wave * each), min(m.y, m.x + (wave + 1) * each), mc, inside, acc);
+        __syncthreads();
+        if (wave > 0)
+#pragma unroll
+            for (int j = 0; j < G; ++j) red[wave - 1][j * 64 + lane] = acc[j];
+        __syncthreads();
+        if (wave == 0 && inside) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) acc[j] = ((acc[j] + red[0][j * 64 + lane]) + red[1][j * 64 + lane]) + red[2][j * 64 + lane];
+            finish_row<DT, G>(dW, into, ldw, m.z, mc, scale, acc);
+        }
+    }
 }
 
 // a workgroup per (chunk, block of columns): the frequent token whose run starts in the chunk, if there is one -- it holds the chunk's last position
 template <int DT, int G>
-__global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__ offsets, const int* __restrict__ token, const float* __restrict__ part, int64_t ldp,
-                                                          char* __restrict__ dW, float* __restrict__ into, int64_t ldw, int D, int V, float scale, int ncb) {
+__global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__ offsets, const int* __restrict__ slot, const float* __restrict__ part, int64_t ldp,
+                                                          char* __restrict__ dW, float* __restrict__ into, int64_t ldw, int D, Owners ow, int slots, float scale, int ncb) {
     __shared__ float red[3][64 * G];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int k = blockIdx.x / ncb, c = ((int)(blockIdx.x % ncb) * 64 + lane) * G;
     const bool in = c < D;
-    const int p0 = k * EMB_LONG, p1 = min(p0 + EMB_LONG, offsets[V]);
+    const int p0 = k * EMB_LONG, p1 = min(p0 + EMB_LONG, offsets[slots]);
     if (p0 >= p1) return;
-    const int v = token[p1 - 1], a = offsets[v], b = offsets[v + 1];
+    const int u = slot[p1 - 1], a = offsets[u], b = offsets[u + 1];
     if (a < p0 || b - a <= EMB_LONG) return;
     const int k1 = (b - 1) / EMB_LONG, n = k1 - k + 1, each = (n + 3) / 4;      // partial sums: slot 0 or 1 of chunk k, slot 0 of the following ones
     const int i0 = min(n, wave * each), i1 = min(n, (wave + 1) * each);
@@ -307,7 +448,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__
     if (wave == 0 && in) {
 #pragma unroll
         for (int j = 0; j < G; ++j) acc[j] = ((acc[j] + red[0][j * 64 + lane]) + red[1][j * 64 + lane]) + red[2][j * 64 + lane];
-        finish_row<DT, G>(dW, into, ldw, v, c, scale, acc);
+        finish_row<DT, G>(dW, into, ldw, ow.token(u), c, scale, acc);
     }
 }
 
@@ -324,10 +465,17 @@ inline int cols_of(int esize, int D, const void* a, int64_t lda, const void* b, 
 }
 
 // one workgroup per CU: each reads every id once, so more of them only multiply the reads
-inline int bins_for(int V) {
-    const int nb = bmt_cdiv(V, 256);
-    return nb < EMB_BINS ? nb : EMB_BINS;
+inline Owners owners_for(int V) {
+    Owners ow = {8, 0};
+    while (bmt_cdiv(V, 1 << ow.lg) > EMB_BINS) ++ow.lg;
+    ow.nb = bmt_cdiv(V, 1 << ow.lg);
+    return ow;
 }
+inline bool splits(int64_t N, const Owners& ow) { return N > EMB_DIRECT && (1 << ow.lg) <= EMB_SPLIT_G; }
+// ids per thread and chunk of the split: at most 256 chunks up to 4 M ids (every workgroup adds up the counts of all chunks)
+inline int split_rounds(int64_t N) { return N <= 256 * 1024 ? 1 : N <= 1024 * 1024 ? 4 : 16; }
+inline int64_t split_chunks(int64_t N) { return (N + 1024 * split_rounds(N) - 1) / (1024 * split_rounds(N)); }
+inline int groups_for(const Owners& ow, int V) { return V < (1 << ow.lg) ? V : 1 << ow.lg; }
 
 #define BMT_EMB_BY(dtype, g, CALL)                                                           \
     do {                                                                                     \
@@ -374,7 +522,10 @@ extern "C" int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, voi
 extern "C" int64_t bmt_embedding_bwd_ws_bytes(int64_t N, int D, int V) {
     if (N < 0 || N > 0x7fffffff - 64 || D <= 0 || V <= 0) return 0;
     const int64_t chunks = (N + EMB_LONG - 1) / EMB_LONG;
-    return round16(((int64_t)V + 1) * 4) + 2 * round16(N * 4) + (N > EMB_LONG ? 2 * chunks * emb_ld(D) * 4 : 0);
+    const Owners ow = owners_for(V);
+    const int64_t G = (int64_t)1 << ow.lg;
+    return round16(((int64_t)groups_for(ow, V) * ow.nb + 1) * 4) + 2 * round16(N * 4) + (N > EMB_FEW ? 2 * chunks * emb_ld(D) * 4 : 0) +
+           (splits(N, ow) ? 2 * round16(N * 4) + round16((G + 1) * 4) + split_chunks(N) * G * 4 : 0);
 }
 
 extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t ld, int64_t N, int D, int V, int dtype, float scale, int64_t pad_idx, void* dW, float* into,
@@ -387,31 +538,46 @@ extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t l
     BMT_CHECK_ARG((ids && dout) || N == 0, "bmt_embedding_bwd: null pointer");
     if (N == 0 && into) return BMT_OK;
     hipStream_t st = (hipStream_t)stream;
+    const Owners ow = owners_for(V);
+    const int groups = groups_for(ow, V), slots = groups * ow.nb;
     int* offsets = (int*)ws;
-    int* order = (int*)((char*)ws + round16(((int64_t)V + 1) * 4));
-    int* token = (int*)((char*)order + round16(N * 4));
-    float* part = (float*)((char*)token + round16(N * 4));
+    int* order = (int*)((char*)ws + round16(((int64_t)slots + 1) * 4));
+    int* slot = (int*)((char*)order + round16(N * 4));
+    float* part = (float*)((char*)slot + round16(N * 4));
     const int es = dtype == BMT_DT_F32 ? 4 : 2;
     const int g = cols_of(es, D, dout, ld, into ? (void*)into : dW, ldw), ncb = bmt_cdiv(D, 64 * g);
-    const int chunks = N > EMB_LONG ? bmt_cdiv(N, EMB_LONG) : 0;      // (fewer positions than that: no token is frequent)
-    const int64_t grid = (int64_t)chunks * ncb + ((int64_t)V * ncb + 3) / 4;
+    const int64_t chunks = N > EMB_FEW ? (N + EMB_LONG - 1) / EMB_LONG : 0;
+    const int64_t grid = chunks * ncb + ((int64_t)V * ncb + 3) / 4;
     const int64_t ldp = emb_ld(D);
     BMT_CHECK_ARG(grid <= 0x7fffffff, "bmt_embedding_bwd: vocabulary too large");
-    const int nb = bins_for(V), groups = bmt_cdiv(V, nb);
-    const size_t lds = (size_t)16 * nb * sizeof(int);
-#define BMT_ORDER(K) hipLaunchKernelGGL((embed_order_kernel<K>), dim3(groups), dim3(1024), lds, st, ids, N, V, pad_idx, nb, offsets, order, token)
-    if (N <= 1024) BMT_ORDER(1);
-    else if (N <= 4096) BMT_ORDER(4);
-    else if (N <= 16384) BMT_ORDER(16);
-    else if (N <= 65536) BMT_ORDER(64);
+    const size_t lds = (size_t)16 * ow.nb * sizeof(int);
+    int bits = 0;
+    while ((1 << bits) < ow.nb) ++bits;
+    Split sp = {};
+    if (splits(N, ow)) {
+        const int64_t G = (int64_t)1 << ow.lg;
+        char* p = (char*)part + 2 * chunks * ldp * 4;
+        sp.pos = (int*)p;
+        sp.key = (int*)(p + round16(N * 4));
+        sp.start = (int*)(p + 2 * round16(N * 4));
+        int* counts = (int*)((char*)sp.start + round16((G + 1) * 4));
+        const int R = split_rounds(N);
+        const unsigned n = (unsigned)split_chunks(N);
+        hipLaunchKernelGGL(embed_count_kernel, dim3(n), dim3(1024), 0, st, ids, N, V, pad_idx, ow, R, counts);
+        hipLaunchKernelGGL(embed_split_kernel, dim3(n), dim3(1024), 0, st, ids, N, V, pad_idx, ow, R, counts, sp);
+    }
+#define BMT_ORDER(K) hipLaunchKernelGGL((embed_order_kernel<K>), dim3(groups), dim3(1024), lds, st, ids, N, V, pad_idx, ow, bits, slots, sp, offsets, order, slot)
+    if (sp.pos) BMT_ORDER(-1);
+    else if (N <= 1024) BMT_ORDER(1);
+    else if (N <= EMB_DIRECT) BMT_ORDER(8);
     else BMT_ORDER(0);
 #undef BMT_ORDER
 #define BMT_CALL(DT, G)                                                                                                                                      \
     do {                                                                                                                                                     \
-        hipLaunchKernelGGL((embed_sum_kernel<DT, G>), dim3((unsigned)grid), dim3(256), 0, st, (const char*)dout, ld, offsets, order, token, part, ldp, (char*)dW, into, ldw, \
-                           D, V, scale, chunks, ncb);                                                                                                        \
-        if (chunks) hipLaunchKernelGGL((embed_join_kernel<DT, G>), dim3((unsigned)(chunks * ncb)), dim3(256), 0, st, offsets, token, part, ldp, (char*)dW, into, ldw, D, V,  \
-                                       scale, ncb);                                                                                                          \
+        hipLaunchKernelGGL((embed_sum_kernel<DT, G>), dim3((unsigned)grid), dim3(256), 0, st, (const char*)dout, ld, offsets, order, slot, part, ldp, (char*)dW, into, ldw, \
+                           D, V, ow, slots, scale, (int)chunks, ncb);                                                                                                        \
+        if (chunks) hipLaunchKernelGGL((embed_join_kernel<DT, G>), dim3((unsigned)(chunks * ncb)), dim3(256), 0, st, offsets, slot, part, ldp, (char*)dW, into, ldw, D, ow, \
+                                       slots, scale, ncb);                                                                                                          \
     } while (0)
     BMT_EMB_BY(dtype, g, BMT_CALL);
 #undef BMT_CALL

@@ -70,6 +70,21 @@ struct Elem<BMT_DT_F16> {
     static __device__ __forceinline__ float get1(const char* p) { return h_bits2f(*reinterpret_cast<const uint16_t*>(p)); }
 };
 
+// e^t, t <= 0 (NaN stays NaN): the instruction's 2^y of y = t log2 e, log2 e as the sum of two floats.  The instruction is right to 2.6e-8 (rms); y's
+// rounding adds 3e-8 |t|
+__device__ __forceinline__ float exp_neg(float t) {
+    return __builtin_amdgcn_exp2f(__fmaf_rn(t, 1.44269502162933349609375f, t * 1.92596299112661746e-8f));
+}
+// the same with what y's rounding lost put back to first order: 2^(y + l) = 2^y (1 + l ln 2), for factors whose error does not average out: 16-bit
+// logits leave few different maxima, every row of a sequence repeats the same few factors, and the errors of hundreds of rows add up (rewards of
+// 1024-token sequences were off by 1.4e-6 of their size; 3e-7 now).  (t = -inf: l is NaN, the median takes it to -1, and 2^y is 0)
+__device__ __forceinline__ float exp_neg_exact(float t) {
+    const float y = t * 1.44269502162933349609375f;
+    const float l = __fmaf_rn(t, 1.92596299112661746e-8f, __fmaf_rn(t, 1.44269502162933349609375f, -y));
+    const float e = __builtin_amdgcn_exp2f(y);
+    return __fmaf_rn(e, __builtin_amdgcn_fmed3f(l, -1.f, 1.f) * 0.693147180559945309f, e);
+}
+
 // the (B, T) rows of a call: logits with two row strides, ids and an optional mask with theirs (all strides in elements)
 struct Rows {
     const char* x;
@@ -87,11 +102,24 @@ struct PolicyIn {
     float lo, hi, beta;
     int reduction;                     // 0 sum, 1 mean over the rows that count, 2 mean over sequences of their means
     int B;
-    const int* counts;                 // [B] rows that count per sequence, [B] their total
+    const int* counts;                 // [B] rows that count per sequence, [B] their total; NULL: every workgroup counts what it needs
 };
 
 __device__ __forceinline__ bool row_counts(const Rows& q, int b, int t, int64_t id) {
     return id != q.pad && (q.mask == nullptr || q.mask[b * q.mb + t * q.mt] != 0);
+}
+
+// the rows a mean divides by (those of sequence b, or all), as this thread's share of a group of NT
+template <int NT>
+__device__ __forceinline__ int count_share(const Rows& q, const PolicyIn& p, int b) {
+    int n = 0;
+    if (p.counts || p.reduction == 0) return 0;
+    if (p.reduction == 2) {
+        for (int t = threadIdx.x; t < q.T; t += NT) n += row_counts(q, b, t, q.id[b * q.ib + t * q.it]);
+    } else {
+        for (int i = threadIdx.x; i < p.B * q.T; i += NT) n += row_counts(q, i / q.T, i % q.T, q.id[(i / q.T) * q.ib + (i % q.T) * q.it]);
+    }
+    return n;
 }
 
 // A row as 16-byte granules of memory: the first one starts at or below the row's first element, so that vector accesses are aligned for every
@@ -165,6 +193,18 @@ __device__ __forceinline__ float group_max(float v, float* red) {
     return m;
 }
 template <int NT>
+__device__ __forceinline__ int group_count(int v, int* red) {      // (red is written once per kernel)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (NT == 64) return v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    int s = red[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) s += red[i];
+    return s;
+}
+template <int NT>
 __device__ __forceinline__ double group_sum(double v, double* red) {
     v = wave_sum_f64(v);
     if constexpr (NT == 64) return v;
@@ -179,7 +219,7 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
 
 // everything a policy row adds to the loss, in 64 bits: the differences of log-probabilities are small beside the values they come from, and the
 // KL term is second order in them.  Returns w_r; terms[0..2] = the row's share of the loss, its KL, whether the clip took its gradient
-__device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, double lp, double* terms) {
+__device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, int counted, double lp, double* terms) {
     const double A = p.adv[b * p.ab + t * p.at];
     const double rho = p.old ? exp(lp - (double)p.old[b * p.ob + t * p.ot]) : exp(lp - lp);      // (lp - lp: NaN stays NaN)
     const double u = rho * A, c = fmin(fmax(rho, 1.0 - (double)p.lo), 1.0 + (double)p.hi) * A;
@@ -192,8 +232,8 @@ __device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, dou
         w -= (double)p.beta * em;
     }
     double norm = 1.0;
-    if (p.reduction == 1) norm = 1.0 / (double)max(p.counts[p.B], 1);
-    else if (p.reduction == 2) norm = 1.0 / ((double)p.B * (double)max(p.counts[b], 1));
+    if (p.reduction == 1) norm = 1.0 / (double)max(p.counts ? p.counts[p.B] : counted, 1);
+    else if (p.reduction == 2) norm = 1.0 / ((double)p.B * (double)max(p.counts ? p.counts[b] : counted, 1));
     terms[0] = loss * norm;
     terms[1] = kl;
     terms[2] = clipped ? 1.0 : 0.0;
@@ -215,7 +255,12 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(Rows q, int B, int* __
     } else {
         for (int b = threadIdx.x >> 6; b < B; b += 16) {
             int n = 0;
-            for (int t = threadIdx.x & 63; t < q.T; t += 64) n += row_counts(q, b, t, q.id[b * q.ib + t * q.it]);
+#pragma unroll 4
+            for (int t = threadIdx.x & 63; t < q.T; t += 64) {
+                const int64_t id = q.id[b * q.ib + t * q.it];
+                const int on = q.mask ? q.mask[b * q.mb + t * q.mt] : 1;
+                n += (id != q.pad) & (on != 0);
+            }
             total += n;
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
@@ -235,18 +280,20 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(Rows q, int B, int* __
 // ---------------------------------------------------------------- forward: statistics and log-probability of every row, any V
 // One sweep with a running maximum and sum per thread.  stats[r] = {max, 1 / sum} for the gradient kernel (0, 0 where the row does not count).
 template <int DT, int NT, bool POLICY>
-__global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float* __restrict__ logp, float2* __restrict__ stats, float* __restrict__ w,
+__global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float* __restrict__ logp, double* __restrict__ logp64, float2* __restrict__ stats, float* __restrict__ w,
                                                         double* __restrict__ terms, int64_t rows) {
     using E = Elem<DT>;
     constexpr int U = 4;
     __shared__ float redf[NT / 64];
     __shared__ double redd[NT / 64];
+    __shared__ int redi[NT / 64];
     const int64_t r = blockIdx.x;
     const int b = (int)(r / q.T), t = (int)(r % q.T);
     const int64_t id = q.id[b * q.ib + t * q.it];
     if (!row_counts(q, b, t, id)) {
         if (threadIdx.x == 0) {
-            logp[r] = 0.f;
+            if (logp) logp[r] = 0.f;
+            if (logp64) logp64[r] = 0.0;
             if (stats) stats[r] = make_float2(0.f, 0.f);
             if constexpr (POLICY) {
                 w[r] = 0.f;
@@ -277,24 +324,27 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
             for (int j = 0; j < E::G; ++j) bm = fmaxf(bm, x[i][j]);
         }
         const float mn = fmaxf(m, bm), ms = mn == -__builtin_huge_valf() ? 0.f : mn;      // (nothing but -inf so far: the sum stays 0)
-        s *= __expf(m - ms);
+        s *= exp_neg(m - ms);
         float a = 0.f;
 #pragma unroll
         for (int i = 0; i < U; ++i)
 #pragma unroll
-            for (int j = 0; j < E::G; ++j) a += __expf(x[i][j] - ms);
+            for (int j = 0; j < E::G; ++j) a += exp_neg(x[i][j] - ms);
         s += a;
         m = mn;
     }
+    int counted = 0;
+    if constexpr (POLICY) counted = group_count<NT>(count_share<NT>(q, p, b), redi);
     const float M = group_max<NT>(m, redf);
-    const double S = group_sum<NT>(m == -__builtin_huge_valf() ? (double)s : (double)s * (double)__expf(m - M), redd);
+    const double S = group_sum<NT>(m == -__builtin_huge_valf() ? (double)s : (double)s * (double)exp_neg_exact(m - M), redd);
     if (threadIdx.x == 0) {
         const double lp = ((double)xt - (double)M) - log(S);
-        logp[r] = (float)lp;
+        if (logp) logp[r] = (float)lp;
+        if (logp64) logp64[r] = lp;
         if (stats) stats[r] = make_float2(M, (float)(1.0 / S));
         if constexpr (POLICY) {
             double tr[3];
-            w[r] = policy_row(p, b, t, lp, tr);
+            w[r] = policy_row(p, b, t, counted, lp, tr);
             terms[r] = tr[0];
             terms[rows + r] = tr[1];
             terms[2 * rows + r] = tr[2];
@@ -310,6 +360,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     using E = Elem<DT>;
     __shared__ float redf[NT / 64];
     __shared__ double redd[NT / 64];
+    __shared__ int redi[NT / 64];
     __shared__ float wc[2];
     const int64_t r = blockIdx.x;
     const int b = (int)(r / q.T), t = (int)(r % q.T);
@@ -346,6 +397,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
 #pragma unroll
         for (int j = 0; j < E::G; ++j) m = fmaxf(m, x[j]);
     }
+    const int counted = group_count<NT>(count_share<NT>(q, p, b), redi);
     m = group_max<NT>(m, redf);
     float s = 0.f;
 #pragma unroll
@@ -354,7 +406,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
             float x[E::G], a = 0.f;
             E::get(v[i], x);
 #pragma unroll
-            for (int j = 0; j < E::G; ++j) a += __expf(x[j] - m);
+            for (int j = 0; j < E::G; ++j) a += exp_neg(x[j] - m);
             s += a;
         }
     }
@@ -362,7 +414,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     if (threadIdx.x == 0) {
         const double lp = ((double)xt - (double)m) - log(S);
         double tr[3];
-        const float wr = policy_row(p, b, t, lp, tr);
+        const float wr = policy_row(p, b, t, counted, lp, tr);
         const float is = (float)(1.0 / S);
         wc[0] = wr;
         wc[1] = is;
@@ -384,7 +436,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
             float x[E::G];
             E::get(v[i], x);
 #pragma unroll
-            for (int j = 0; j < E::G; ++j) x[j] = __expf(x[j] - m) * c;
+            for (int j = 0; j < E::G; ++j) x[j] = exp_neg(x[j] - m) * c;
             if (k == kt) {
 #pragma unroll
                 for (int j = 0; j < E::G; ++j)
@@ -396,25 +448,30 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
 }
 
 // loss[0] = sum of the rows' shares, info[0] = mean KL, info[1] = share of rows whose gradient the clip took (means over the rows that count)
-__global__ __launch_bounds__(1024) void policy_finish_kernel(const double* __restrict__ terms, int64_t rows, const int* __restrict__ total, float* __restrict__ loss,
+__global__ __launch_bounds__(1024) void policy_finish_kernel(const double* __restrict__ terms, const float2* __restrict__ stats, int64_t rows, float* __restrict__ loss,
                                                               float* __restrict__ info) {
-    __shared__ double red[3][16];
-    double a[3] = {0.0, 0.0, 0.0};
-    for (int64_t r = threadIdx.x; r < rows; r += 1024)
+    __shared__ double red[4][16];
+    double a[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
 #pragma unroll
         for (int k = 0; k < 3; ++k) a[k] += terms[k * rows + r];
+        a[3] += stats[r].y == 0.f ? 0.0 : 1.0;      // (a row that counts has a finite sum)
+    }
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < 4; ++k) {
         a[k] = wave_sum_f64(a[k]);
         if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = a[k];
     }
     __syncthreads();
     if (threadIdx.x < 3) {
-        double v = 0.0;
-        for (int i = 0; i < 16; ++i) v += red[threadIdx.x][i];
-        const double n = (double)max(total[0], 1);
+        double v = 0.0, n = 0.0;
+        for (int i = 0; i < 16; ++i) {
+            v += red[threadIdx.x][i];
+            n += red[3][i];
+        }
         if (threadIdx.x == 0) loss[0] = (float)v;
-        else info[threadIdx.x - 1] = (float)(v / n);
+        else info[threadIdx.x - 1] = (float)(v / fmax(n, 1.0));
     }
 }
 
@@ -426,7 +483,8 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
     using E = Elem<DT>;
     const float gs = g ? g[0] : 1.f;
     if (once && gs == 1.f) return;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+        const int64_t r = rows - 1 - i;      // last rows first: what the forward pass read last is what the memory-side cache still holds
         const int b = (int)(r / q.T), t = (int)(r % q.T);
         const int64_t id = q.id[b * q.ib + t * q.it];
         const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
@@ -446,7 +504,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
             float x[E::G];
             E::get(row.load(k), x);
 #pragma unroll
-            for (int j = 0; j < E::G; ++j) x[j] = __expf(x[j] - m) * c;
+            for (int j = 0; j < E::G; ++j) x[j] = exp_neg(x[j] - m) * c;
             if (k == kt) {
 #pragma unroll
                 for (int j = 0; j < E::G; ++j)
@@ -461,51 +519,54 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
 __device__ __forceinline__ double softplus64(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 __device__ __forceinline__ double sigmoid64(double x) { return 1.0 / (1.0 + exp(-x)); }
 
-__global__ __launch_bounds__(1024) void preference_pairs_kernel(const float* __restrict__ logp, const float2* __restrict__ stats, int P, int T, const float* __restrict__ ref,
+constexpr int PAIRS_WG = 128;      // most pairs of one workgroup (their sums stand in LDS)
+
+// workgroup g: pairs [g * each, ..).  A wave adds up a sequence, then a thread works out a pair.  gridDim.x == 1: loss[0], else part[g] (sum_f64_kernel)
+__global__ __launch_bounds__(1024) void preference_pairs_kernel(const double* __restrict__ logp, const float2* __restrict__ stats, int P, int T, int each, const float* __restrict__ ref,
                                                                  int64_t rs, float beta, float smoothing, int mean, float* __restrict__ rewards, float* __restrict__ w,
-                                                                 double* __restrict__ pair_loss, float* __restrict__ loss) {
-    __shared__ double red[16];
-    const int lane = threadIdx.x & 63;
-    double acc = 0.0;
-    for (int i = blockIdx.x * 16 + (threadIdx.x >> 6); i < P; i += gridDim.x * 16) {
-        double S[2], len[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t r0 = (int64_t)(i + h * P) * T;
-            double a = 0.0, c = 0.0;
-            for (int t = lane; t < T; t += 64) {
-                a += (double)logp[r0 + t];
-                c += stats[r0 + t].y == 0.f ? 0.0 : 1.0;      // (a row that counts has a finite sum)
-            }
-            S[h] = wave_sum_f64(a);
-            len[h] = fmax(wave_sum_f64(c), 1.0);
+                                                                 double* __restrict__ part, float* __restrict__ loss) {
+    __shared__ double sum[2][PAIRS_WG], len[2][PAIRS_WG], red[16];
+    const int lane = threadIdx.x & 63, p0 = blockIdx.x * each, n = min(each, P - p0);
+    for (int j = threadIdx.x >> 6; j < 2 * n; j += 16) {
+        const int h = j >= n, i = j - h * n;
+        const int64_t r0 = (int64_t)(p0 + i + h * P) * T;
+        double a = 0.0, c = 0.0;
+#pragma unroll 4
+        for (int t = lane; t < T; t += 64) {
+            a += logp[r0 + t];
+            if (mean) c += stats[r0 + t].y == 0.f ? 0.0 : 1.0;      // (a row that counts has a finite sum)
         }
-        const double i0 = mean ? 1.0 / len[0] : 1.0, i1 = mean ? 1.0 / len[1] : 1.0;
-        const double r0 = (double)beta * (S[0] * i0 - (double)ref[(int64_t)i * rs]), r1 = (double)beta * (S[1] * i1 - (double)ref[(int64_t)(i + P) * rs]);
+        a = wave_sum_f64(a);
+        c = wave_sum_f64(c);
+        if (lane == 0) {
+            sum[h][i] = a;
+            len[h][i] = mean ? fmax(c, 1.0) : 1.0;
+        }
+    }
+    __syncthreads();
+    double l = 0.0;
+    if ((int)threadIdx.x < n) {
+        const int i = threadIdx.x, g = p0 + i;
+        const double i0 = 1.0 / len[0][i], i1 = 1.0 / len[1][i];
+        const double r0 = (double)beta * (sum[0][i] * i0 - (double)ref[(int64_t)g * rs]), r1 = (double)beta * (sum[1][i] * i1 - (double)ref[(int64_t)(g + P) * rs]);
         const double z = r0 - r1, ls = (double)smoothing;
-        double l = (1.0 - ls) * softplus64(-z), d = (1.0 - ls) * sigmoid64(-z);
+        l = (1.0 - ls) * softplus64(-z);
+        double d = (1.0 - ls) * sigmoid64(-z);
         if (ls != 0.0) {      // (0 * inf)
             l += ls * softplus64(z);
             d -= ls * sigmoid64(z);
         }
+        l /= (double)P;
         d *= -(double)beta / (double)P;
-        if (lane == 0) {
-            rewards[i] = (float)r0;
-            rewards[i + P] = (float)r1;
-            if (w) {
-                w[i] = (float)(d * i0);
-                w[i + P] = (float)(-d * i1);
-            }
-            if (pair_loss) pair_loss[i] = l / (double)P;
-        }
-        acc += l / (double)P;
+        rewards[g] = (float)r0;
+        rewards[g + P] = (float)r1;
+        w[g] = (float)(d * i0);
+        w[g + P] = (float)(-d * i1);
     }
-    if (gridDim.x > 1) return;      // (sum_f64_kernel adds pair_loss)
-    if (lane == 0) red[threadIdx.x >> 6] = acc;
-    __syncthreads();
+    l = group_sum<1024>(l, red);
     if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; ++k) acc += red[k];
-        loss[0] = (float)acc;
+        if (gridDim.x == 1) loss[0] = (float)l;
+        else part[blockIdx.x] = l;
     }
 }
 
@@ -535,13 +596,13 @@ inline int threads_for(int64_t rows, int64_t granules) {
 }
 
 template <int DT>
-void launch_logp(const Rows& q, const PolicyIn* p, float* logp, float2* stats, float* w, double* terms, int64_t rows, hipStream_t st) {
+void launch_logp(const Rows& q, const PolicyIn* p, float* logp, double* logp64, float2* stats, float* w, double* terms, int64_t rows, hipStream_t st) {
     const int nt = threads_for(rows, ((int64_t)q.V + Elem<DT>::G - 1) / Elem<DT>::G);
     const PolicyIn none = {};
 #define BMT_ROWS(NT)                                                                                                                               \
     do {                                                                                                                                           \
-        if (p) hipLaunchKernelGGL((logp_rows_kernel<DT, NT, true>), dim3((unsigned)rows), dim3(NT), 0, st, q, *p, logp, stats, w, terms, rows);      \
-        else hipLaunchKernelGGL((logp_rows_kernel<DT, NT, false>), dim3((unsigned)rows), dim3(NT), 0, st, q, none, logp, stats, w, terms, rows);     \
+        if (p) hipLaunchKernelGGL((logp_rows_kernel<DT, NT, true>), dim3((unsigned)rows), dim3(NT), 0, st, q, *p, logp, logp64, stats, w, terms, rows);      \
+        else hipLaunchKernelGGL((logp_rows_kernel<DT, NT, false>), dim3((unsigned)rows), dim3(NT), 0, st, q, none, logp, logp64, stats, w, terms, rows);     \
     } while (0)
     if (nt == 64) BMT_ROWS(64);
     else if (nt == 256) BMT_ROWS(256);
@@ -601,7 +662,7 @@ extern "C" int bmt_logp_rows(const void* logits, int dtype, int64_t sb, int64_t 
     if (rows == 0) return BMT_OK;
     BMT_CHECK_ARG(logp, "bmt_logp_rows: null pointer");
     const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
-#define BMT_CALL(DT) launch_logp<DT>(q, nullptr, logp, (float2*)stats, nullptr, nullptr, rows, (hipStream_t)stream)
+#define BMT_CALL(DT) launch_logp<DT>(q, nullptr, logp, nullptr, (float2*)stats, nullptr, nullptr, rows, (hipStream_t)stream)
     BMT_BY_DTYPE(dtype, BMT_CALL);
 #undef BMT_CALL
     BMT_CHECK_LAUNCH("bmt_logp_rows");
@@ -650,29 +711,31 @@ extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_
     float2* stats = (float2*)(terms + 3 * rows);
     float* w = (float*)(stats + rows);
     int* counts = (int*)(w + rows);
+    // what a mean divides by: a few thousand ids are counted by every row's workgroup beside its loads (a launch less), more by one of their own
+    const int64_t divides = reduction == 0 ? 0 : reduction == 1 ? rows : T;
     const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
-    const PolicyIn p = {old_logp, ref_logp, adv, ob, ot, rb, rt, ab, at, clip_low, clip_high, kl_coef, reduction, B, counts};
-    hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, s, q, B, counts);
+    const PolicyIn p = {old_logp, ref_logp, adv, ob, ot, rb, rt, ab, at, clip_low, clip_high, kl_coef, reduction, B, divides > 2048 ? counts : nullptr};
+    if (divides > 2048) hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, s, q, B, counts);
     bool done = false;
 #define BMT_CALL(DT) done = launch_policy<DT>(q, p, dlogits, db, dt, logp, stats, w, terms, rows, s)
     if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
 #undef BMT_CALL
     if (!done) {      // no gradient wanted, or rows too long for the registers: a second read
-#define BMT_CALL(DT) launch_logp<DT>(q, &p, logp, stats, w, terms, rows, s)
+#define BMT_CALL(DT) launch_logp<DT>(q, &p, logp, nullptr, stats, w, terms, rows, s)
         BMT_BY_DTYPE(dtype, BMT_CALL);
 #undef BMT_CALL
 #define BMT_CALL(DT) launch_grad<DT>(q, stats, w, T, 1, nullptr, 0, dlogits, db, dt, rows, s)
         if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
 #undef BMT_CALL
     }
-    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, s, terms, rows, counts + B, loss, info);
+    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, s, terms, stats, rows, loss, info);
     BMT_CHECK_LAUNCH("bmt_policy_loss");
     return BMT_OK;
 }
 
 extern "C" int64_t bmt_preference_ws_bytes(int B, int T) {
     if (B < 0 || T < 0) return 0;
-    return (int64_t)B * T * (2 * 4 + 4) + (int64_t)B * 4 + 8 + (int64_t)(B / 2) * 8;
+    return (int64_t)B * T * (8 + 8) + (int64_t)(B + 1) / 2 * 8 + (int64_t)(B / 2) * 8;
 }
 
 extern "C" int bmt_preference_loss(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it, const uint8_t* mask,
@@ -687,19 +750,21 @@ extern "C" int bmt_preference_loss(const void* logits, int dtype, int64_t sb, in
     BMT_CHECK_ARG(ws_bytes >= bmt_preference_ws_bytes(B, T) && (reinterpret_cast<uintptr_t>(ws) & 7) == 0,
                   "bmt_preference_loss: workspace of %lld bytes is too small or not aligned", (long long)ws_bytes);
     hipStream_t s = (hipStream_t)stream;
-    // workspace: stats [rows][2] | w [B] | logp [rows] | pad to 8 | pair losses [B / 2] (64-bit)
+    // workspace: stats [rows][2] | w [B] (pad to 8 bytes) | logp [rows] (64-bit: rewards are small differences of long sums) | pair losses [B / 2]
     float2* stats = (float2*)ws;
     float* w = (float*)(stats + rows);
-    float* logp = w + B;
-    double* pair = (double*)((char*)ws + (rows * 12 + (int64_t)B * 4 + 7) / 8 * 8);
+    double* logp = (double*)(stats + rows + (B + 1) / 2);
+    double* pair = logp + rows;
     const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
-#define BMT_CALL(DT) launch_logp<DT>(q, nullptr, logp, stats, nullptr, nullptr, rows, s)
+#define BMT_CALL(DT) launch_logp<DT>(q, nullptr, nullptr, logp, stats, nullptr, nullptr, rows, s)
     BMT_BY_DTYPE(dtype, BMT_CALL);
 #undef BMT_CALL
-    const int pairs = B / 2, blocks = pairs <= 128 ? 1 : bmt_cdiv(pairs, 16);      // one workgroup (8 pairs a wave) adds its own losses
-    hipLaunchKernelGGL(preference_pairs_kernel, dim3(blocks), dim3(1024), 0, s, logp, stats, pairs, T, ref_logp, ref_stride, beta, smoothing, mean_logp, rewards, w,
-                       blocks > 1 ? pair : nullptr, loss);
-    if (blocks > 1) hipLaunchKernelGGL(sum_f64_kernel, dim3(1), dim3(1024), 0, s, pair, (int64_t)pairs, loss);
+    // one workgroup does it all while its waves have at most 16 batches of 256 rows to add (about 8 us); beyond, 8 pairs -- a wave per sequence -- each
+    const int pairs = B / 2;
+    const bool one = pairs <= PAIRS_WG && (int64_t)bmt_cdiv(2 * pairs, 16) * bmt_cdiv(T, 256) <= 16;
+    const int each = one ? pairs : 8, blocks = bmt_cdiv(pairs, each);
+    hipLaunchKernelGGL(preference_pairs_kernel, dim3(blocks), dim3(1024), 0, s, logp, stats, pairs, T, each, ref_logp, ref_stride, beta, smoothing, mean_logp, rewards, w, pair, loss);
+    if (blocks > 1) hipLaunchKernelGGL(sum_f64_kernel, dim3(1), dim3(1024), 0, s, pair, (int64_t)blocks, loss);
     BMT_CHECK_LAUNCH("bmt_preference_loss");
     return BMT_OK;
 }

@@ -3600,30 +3600,30 @@ def mask_from_tokens(trg: torch.Tensor, pad_idx: int, want_src: bool = True, wan
 # (kernels: csrc/tuning_loss.hip, csrc/embedding.hip)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # BMT_DT_*
 _NO_PAD = -(1 << 63)
+# the handle of a device's current stream.  (current_stream() builds a Stream object around it: 2 us of a 10 us call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _tuning_device(who: str, *tensors) -> torch.device:
-    """the one device all the tensors (None: absent) are on"""
-    dev = None
+def _tuning_device(who: str, *tensors):
+    """refuses tensors (None: absent) that are not all on one GPU"""
+    dev = tensors[0].device
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"{who}: bmt_amd ops need CUDA/HIP tensors: there is no CPU fallback (use the oracle for CPU checks)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if t.device != dev:
             raise ValueError(f"{who}: tensors on {dev} and {t.device}")
-    return dev
 
 
 def _run_on(dev: torch.device, what: str, fn, *args):
     """fn(*args, stream) on the current stream of ``dev``, which need not be the current device"""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    i = dev.index
+    if torch.cuda.current_device() == i:
+        rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(i))
     if rc != 0:
         _lib.check(rc, what)
 
@@ -3727,18 +3727,22 @@ def token_logp(logits, ids, mask=None, pad_idx: Optional[int] = None):
 class PolicyStats:
     """what policy_loss saw: ``logp`` (B, T) of the tokens (0 where a row does not count), and the means over the rows that count of the KL term
     (0 without a reference) and of the rows whose gradient the clip took -- device values, no graph"""
-    __slots__ = ("logp", "_info")
+    __slots__ = ("_buf", "_shape")
 
-    def __init__(self, logp, info):
-        self.logp, self._info = logp, info
+    def __init__(self, buf, shape):
+        self._buf, self._shape = buf, shape          # KL, clip fraction, log-probabilities
 
     @property
     def kl(self):
-        return self._info[0]
+        return self._buf[0]
 
     @property
     def clip_fraction(self):
-        return self._info[1]
+        return self._buf[1]
+
+    @property
+    def logp(self):
+        return self._buf[2:].view(self._shape)
 
 
 _REDUCTIONS = {"sum": 0, "token": 1, "sequence": 2}
@@ -3754,8 +3758,7 @@ class PolicyLossFn(torch.autograd.Function):
         B, T, V = x.shape
         dev = x.device
         loss = torch.empty((), device=dev, dtype=torch.float32)
-        info = torch.empty(2, device=dev, dtype=torch.float32)
-        logp = torch.empty(B, T, device=dev, dtype=torch.float32)
+        info = torch.empty(2 + B * T, device=dev, dtype=torch.float32)
         n = lib.bmt_policy_ws_bytes(B, T)
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
         d = _logit_grad_buffer(x) if ctx.needs_input_grad[0] else None
@@ -3765,17 +3768,17 @@ class PolicyLossFn(torch.autograd.Function):
         adv, ab, at = _per_row("policy_loss", "advantages", adv, B, T, per_sequence=True)
         _run_on(dev, "bmt_policy_loss", lib.bmt_policy_loss, *_row_args(x, ids, mask, pad_idx), None if old is None else old.data_ptr(), ob, ot,
                 None if ref is None else ref.data_ptr(), rb, rt, adv.data_ptr(), ab, at, lo, hi, beta, reduction, loss.data_ptr(), info.data_ptr(),
-                logp.data_ptr(), ws.data_ptr(), n, None if d is None else d.data_ptr(), db, dt)
+                info.data_ptr() + 8, ws.data_ptr(), n, None if d is None else d.data_ptr(), db, dt)
         if d is not None:
             ctx.save_for_backward(x, ids, mask, ws)
             ctx.pad_idx, ctx.dlogits = pad_idx, d
-        ctx.mark_non_differentiable(info, logp)
+        ctx.mark_non_differentiable(info)
         ctx.set_materialize_grads(False)
-        return loss, info, logp
+        return loss, info
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, g, _info, _logp):
+    def backward(ctx, g, _info):
         if g is None:
             return (None,) * 11
         x, ids, mask, ws = ctx.saved_tensors
@@ -3803,9 +3806,9 @@ def policy_loss(logits, ids, old_logp, advantages, ref_logp=None, mask=None, pad
         raise ValueError(f"policy_loss: clip range ({clip_low}, {clip_high})")
     if advantages is None:
         raise ValueError("policy_loss: advantages are needed")
-    loss, info, logp = PolicyLossFn.apply(logits, ids, old_logp, advantages, ref_logp, mask, pad_idx, float(clip_low), float(clip_high), float(kl_coef),
-                                          _REDUCTIONS[reduction])
-    return loss, PolicyStats(logp, info)
+    loss, info = PolicyLossFn.apply(logits, ids, old_logp, advantages, ref_logp, mask, pad_idx, float(clip_low), float(clip_high), float(kl_coef),
+                                    _REDUCTIONS[reduction])
+    return loss, PolicyStats(info, ids.shape)
 
 
 class PreferenceLossFn(torch.autograd.Function):
@@ -3879,16 +3882,20 @@ class EmbeddingFn(torch.autograd.Function):
         (ids,) = ctx.saved_tensors
         (V, D), scale, pad_idx = ctx.meta
         n = ids.numel()
-        d2 = dy.reshape(n, D)
-        if D > 1 and d2.stride(1) != 1:
-            d2 = d2.contiguous()
+        if dy.is_contiguous():
+            d2, ld = dy, D
+        else:
+            d2 = dy.reshape(n, D)
+            if D > 1 and d2.stride(1) != 1:
+                d2 = d2.contiguous()
+            ld = d2.stride(0)
         gW = static_grad(ctx.weight)
         if gW is not None and (gW.shape != (V, D) or gW.dtype != torch.float32 or d2.dtype != torch.float32):
             gW = None
         dW = torch.empty(V, D, device=dy.device, dtype=dy.dtype) if gW is None else None
         nws = lib.bmt_embedding_bwd_ws_bytes(n, D, V)
         ws = torch.empty(nws, device=dy.device, dtype=torch.uint8)
-        _run_on(dy.device, "bmt_embedding_bwd", lib.bmt_embedding_bwd, ids.data_ptr(), d2.data_ptr(), d2.stride(0), n, D, V, _DTYPES[dy.dtype], scale,
+        _run_on(dy.device, "bmt_embedding_bwd", lib.bmt_embedding_bwd, ids.data_ptr(), d2.data_ptr(), ld, n, D, V, _DTYPES[dy.dtype], scale,
                 _NO_PAD if pad_idx is None else int(pad_idx), None if dW is None else dW.data_ptr(), None if gW is None else gW.data_ptr(), D, ws.data_ptr(), nws)
         if gW is not None:
             grad_done(ctx.weight)
