@@ -81,7 +81,7 @@ struct Cols {
 #pragma unroll
             for (int j = 0; j < G / 2; ++j) v[j] = pack_2<DT == BMT_DT_F16>(x[2 * j], x[2 * j + 1]);
         }
-        *reinterpret_cast<T*>(p) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<T*>(p));
     }
 };
 
@@ -303,29 +303,33 @@ __global__ __launch_bounds__(1024) void embed_split_kernel(const int64_t* __rest
     }
 }
 
-// rows order[p0 .. p1) of dout, columns c .. c + G, added in order; a lane outside the columns adds nothing
-template <int DT, int G>
-__device__ __forceinline__ void add_rows(const char* dout, int64_t ld, const int* __restrict__ order, int p0, int p1, int c, bool in, float (&acc)[G]) {
-    constexpr int E = elem_size<DT>(), U = 8;
+// rows order[p0 .. p1) of dout, NB blocks of 64 G columns from c on, added in order; a lane outside the columns adds nothing
+template <int DT, int G, int NB>
+__device__ __forceinline__ void add_rows(const char* dout, int64_t ld, const int* __restrict__ order, int p0, int p1, int c, int D, float (&acc)[NB][G]) {
+    constexpr int E = elem_size<DT>(), U = 8 / NB;
     const int lane = threadIdx.x & 63;
     for (int p = p0; p < p1; p += 64) {
         const int have = min(64, p1 - p);
         const int pos = lane < have ? order[p + lane] : 0;
         for (int i = 0; i < have; i += U) {
-            typename Cols<DT, G>::T v[U];
+            typename Cols<DT, G>::T v[U][NB];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int n = __builtin_amdgcn_readlane(pos, min(i + u, have - 1));
-                if (in && i + u < have) v[u] = Cols<DT, G>::load(dout + ((int64_t)n * ld + c) * E);
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    if (c + j * 64 * G < D && i + u < have) v[u][j] = Cols<DT, G>::load(dout + ((int64_t)n * ld + c + j * 64 * G) * E);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (in && i + u < have) {
-                    float x[G];
-                    Cols<DT, G>::get(v[u], x);
 #pragma unroll
-                    for (int j = 0; j < G; ++j) acc[j] += x[j];
-                }
+                for (int j = 0; j < NB; ++j)
+                    if (c + j * 64 * G < D && i + u < have) {
+                        float x[G];
+                        Cols<DT, G>::get(v[u][j], x);
+#pragma unroll
+                        for (int k = 0; k < G; ++k) acc[j][k] += x[k];
+                    }
         }
     }
 }
@@ -345,17 +349,34 @@ __device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, i
     Cols<DT, G>::store(dW + ((int64_t)v * ldw + c) * elem_size<DT>(), x);
 }
 
-// workgroups [0, chunks * ncb): partial sums of the frequent tokens; behind them: a wave per (token, block of columns)
-template <int DT, int G>
+// the four waves' sums into wave 0, in order
+template <int G, int NB>
+__device__ __forceinline__ void join_waves(float (&acc)[NB][G], float (&red)[3][NB][64 * G], int wave, int lane) {
+    __syncthreads();
+    if (wave > 0)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int g = 0; g < G; ++g) red[wave - 1][j][g * 64 + lane] = acc[j][g];
+    __syncthreads();
+    if (wave == 0)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int g = 0; g < G; ++g) acc[j][g] = ((acc[j][g] + red[0][j][g * 64 + lane]) + red[1][j][g * 64 + lane]) + red[2][j][g * 64 + lane];
+}
+
+// workgroups [0, chunks * ncb): partial sums of the frequent tokens; behind them: a wave per (token, NB blocks of columns) -- two where a row has
+// them, so that a wave's way to its first row (offsets, positions) is paid once per row
+template <int DT, int G, int NB>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__ dout, int64_t ld, const int* __restrict__ offsets, const int* __restrict__ order,
                                                          const int* __restrict__ slot, float* __restrict__ part, int64_t ldp, char* __restrict__ dW,
                                                          float* __restrict__ into, int64_t ldw, int D, int V, Owners ow, int slots, float scale, int chunks, int ncb) {
-    __shared__ float red[3][64 * G];
+    __shared__ float red[3][NB][64 * G];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t wg = blockIdx.x, nlong = (int64_t)chunks * ncb;
     if (wg < nlong) {
-        const int k = (int)(wg / ncb), c = ((int)(wg % ncb) * 64 + lane) * G;
-        const bool in = c < D;
+        const int k = (int)(wg / ncb), c = ((int)(wg % ncb) * NB * 64 + lane) * G;
         const int p0 = k * EMB_LONG, p1 = min(p0 + EMB_LONG, offsets[slots]);
         if (p0 >= p1) return;
         const int t0 = slot[p0], t1 = slot[p1 - 1];
@@ -366,31 +387,31 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
             const int a = offsets[u], b = offsets[u + 1];
             if (b - a <= EMB_LONG) continue;
             const int q0 = max(p0, a), q1 = min(p1, b), each = (q1 - q0 + 3) / 4;
-            float acc[G] = {};
-            add_rows<DT, G>(dout, ld, order, min(q1, q0 + wave * each), min(q1, q0 + (wave + 1) * each), c, in, acc);
-            __syncthreads();
-            if (wave > 0)
+            float acc[NB][G] = {};
+            add_rows<DT, G, NB>(dout, ld, order, min(q1, q0 + wave * each), min(q1, q0 + (wave + 1) * each), c, D, acc);
+            join_waves<G, NB>(acc, red, wave, lane);
+            if (wave == 0)
 #pragma unroll
-                for (int j = 0; j < G; ++j) red[wave - 1][j * 64 + lane] = acc[j];
-            __syncthreads();
-            if (wave == 0 && in) {
-                float* o = part + (int64_t)(2 * k + h) * ldp + c;
+                for (int j = 0; j < NB; ++j)
+                    if (c + j * 64 * G < D) {
+                        float* o = part + (int64_t)(2 * k + h) * ldp + c + j * 64 * G;
 #pragma unroll
-                for (int j = 0; j < G; ++j) o[j] = ((acc[j] + red[0][j * 64 + lane]) + red[1][j * 64 + lane]) + red[2][j * 64 + lane];
-            }
+                        for (int g = 0; g < G; ++g) o[g] = acc[j][g];
+                    }
         }
         return;
     }
     const int64_t task = (wg - nlong) * 4 + wave;
     const bool have = task < (int64_t)V * ncb;
-    const int v = have ? (int)(task / ncb) : 0, c = ((int)(task % ncb) * 64 + lane) * G;
-    const bool in = c < D;
+    const int v = have ? (int)(task / ncb) : 0, c = ((int)(task % ncb) * NB * 64 + lane) * G;
     const int u = ow.slot(v), a = offsets[u], b = have ? offsets[u + 1] : a;
     const bool rare = b - a <= EMB_LONG;
     if (rare && have && !(into && a == b)) {
-        float acc[G] = {};
-        add_rows<DT, G>(dout, ld, order, a, b, c, in, acc);
-        if (in) finish_row<DT, G>(dW, into, ldw, v, c, scale, acc);
+        float acc[NB][G] = {};
+        add_rows<DT, G, NB>(dout, ld, order, a, b, c, D, acc);
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (c + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, v, c + j * 64 * G, scale, acc[j]);
     }
     if (chunks) return;
     // no partial sums: the four waves share each frequent token that one of them met
@@ -401,20 +422,14 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
     for (int t = 0; t < 4; ++t) {
         const int4 m = met[t];
         if (m.x == m.y) continue;
-        const int mc = (m.w * 64 + lane) * G, each = (m.y - m.x + 3) / 4;
-        const bool inside = mc < D;
-        float acc[G] = {};
-        add_rows<DT, G>(dout, ld, order, min(m.y, m.x + wave * each), min(m.y, m.x + (wave + 1) * each), mc, inside, acc);
-        __syncthreads();
-        if (wave > 0)
+        const int mc = (m.w * NB * 64 + lane) * G, each = (m.y - m.x + 3) / 4;
+        float acc[NB][G] = {};
+        add_rows<DT, G, NB>(dout, ld, order, min(m.y, m.x + wave * each), min(m.y, m.x + (wave + 1) * each), mc, D, acc);
+        join_waves<G, NB>(acc, red, wave, lane);
+        if (wave == 0)
 #pragma unroll
-            for (int j = 0; j < G; ++j) red[wave - 1][j * 64 + lane] = acc[j];
-        __syncthreads();
-        if (wave == 0 && inside) {
-#pragma unroll
-            for (int j = 0; j < G; ++j) acc[j] = ((acc[j] + red[0][j * 64 + lane]) + red[1][j * 64 + lane]) + red[2][j * 64 + lane];
-            finish_row<DT, G>(dW, into, ldw, m.z, mc, scale, acc);
-        }
+            for (int j = 0; j < NB; ++j)
+                if (mc + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, m.z, mc + j * 64 * G, scale, acc[j]);
     }
 }
 
@@ -422,7 +437,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
 template <int DT, int G>
 __global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__ offsets, const int* __restrict__ slot, const float* __restrict__ part, int64_t ldp,
                                                           char* __restrict__ dW, float* __restrict__ into, int64_t ldw, int D, Owners ow, int slots, float scale, int ncb) {
-    __shared__ float red[3][64 * G];
+    __shared__ float red[3][1][64 * G];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int k = blockIdx.x / ncb, c = ((int)(blockIdx.x % ncb) * 64 + lane) * G;
     const bool in = c < D;
@@ -432,24 +447,17 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__
     if (a < p0 || b - a <= EMB_LONG) return;
     const int k1 = (b - 1) / EMB_LONG, n = k1 - k + 1, each = (n + 3) / 4;      // partial sums: slot 0 or 1 of chunk k, slot 0 of the following ones
     const int i0 = min(n, wave * each), i1 = min(n, (wave + 1) * each);
-    float acc[G] = {};
+    float acc[1][G] = {};
     if (in) {
 #pragma unroll 4
         for (int i = i0; i < i1; ++i) {
             const float* o = part + (int64_t)(2 * (k + i) + (i == 0 && a > p0 ? 1 : 0)) * ldp + c;
 #pragma unroll
-            for (int j = 0; j < G; ++j) acc[j] += o[j];
+            for (int j = 0; j < G; ++j) acc[0][j] += o[j];
         }
     }
-    if (wave > 0)
-#pragma unroll
-        for (int j = 0; j < G; ++j) red[wave - 1][j * 64 + lane] = acc[j];
-    __syncthreads();
-    if (wave == 0 && in) {
-#pragma unroll
-        for (int j = 0; j < G; ++j) acc[j] = ((acc[j] + red[0][j * 64 + lane]) + red[1][j * 64 + lane]) + red[2][j * 64 + lane];
-        finish_row<DT, G>(dW, into, ldw, ow.token(u), c, scale, acc);
-    }
+    join_waves<G, 1>(acc, red, wave, lane);
+    if (wave == 0 && in) finish_row<DT, G>(dW, into, ldw, ow.token(u), c, scale, acc[0]);
 }
 
 inline int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -545,9 +553,9 @@ extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t l
     int* slot = (int*)((char*)order + round16(N * 4));
     float* part = (float*)((char*)slot + round16(N * 4));
     const int es = dtype == BMT_DT_F32 ? 4 : 2;
-    const int g = cols_of(es, D, dout, ld, into ? (void*)into : dW, ldw), ncb = bmt_cdiv(D, 64 * g);
+    const int g = cols_of(es, D, dout, ld, into ? (void*)into : dW, ldw), ncb = bmt_cdiv(D, 64 * g), nb2 = ncb >= 2 ? 2 : 1, ncs = bmt_cdiv(ncb, nb2);
     const int64_t chunks = N > EMB_FEW ? (N + EMB_LONG - 1) / EMB_LONG : 0;
-    const int64_t grid = chunks * ncb + ((int64_t)V * ncb + 3) / 4;
+    const int64_t grid = chunks * ncs + ((int64_t)V * ncs + 3) / 4;
     const int64_t ldp = emb_ld(D);
     BMT_CHECK_ARG(grid <= 0x7fffffff, "bmt_embedding_bwd: vocabulary too large");
     const size_t lds = (size_t)16 * ow.nb * sizeof(int);
@@ -574,8 +582,10 @@ extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t l
 #undef BMT_ORDER
 #define BMT_CALL(DT, G)                                                                                                                                      \
     do {                                                                                                                                                     \
-        hipLaunchKernelGGL((embed_sum_kernel<DT, G>), dim3((unsigned)grid), dim3(256), 0, st, (const char*)dout, ld, offsets, order, slot, part, ldp, (char*)dW, into, ldw, \
-                           D, V, ow, slots, scale, (int)chunks, ncb);                                                                                                        \
+        if (nb2 == 2) hipLaunchKernelGGL((embed_sum_kernel<DT, G, 2>), dim3((unsigned)grid), dim3(256), 0, st, (const char*)dout, ld, offsets, order, slot, part, ldp,          \
+                                         (char*)dW, into, ldw, D, V, ow, slots, scale, (int)chunks, ncs);                                                    \
+        else hipLaunchKernelGGL((embed_sum_kernel<DT, G, 1>), dim3((unsigned)grid), dim3(256), 0, st, (const char*)dout, ld, offsets, order, slot, part, ldp, (char*)dW, into, \
+                                ldw, D, V, ow, slots, scale, (int)chunks, ncs);                                                                              \
         if (chunks) hipLaunchKernelGGL((embed_join_kernel<DT, G>), dim3((unsigned)(chunks * ncb)), dim3(256), 0, st, offsets, slot, part, ldp, (char*)dW, into, ldw, D, ow, \
                                        slots, scale, ncb);                                                                                                          \
     } while (0)

@@ -3,9 +3,11 @@
 // over any number of fp32 / bf16 / fp16 tensors (s: an optional scale of all gradients that the caller has not applied yet).
 // Bound: HBM -- the norm reads every gradient once, and nothing can be written before it is known, so clipping reads them a second time.
 // Two launches: `norm` leaves one 64-bit partial sum per workgroup; every workgroup of `apply` adds those (they come from L2), in one order, and
-// scales its tiles, walking them backwards: the tiles the norm read last are the ones the memory-side cache still holds.
-// Squares and sums are 64-bit: a product of two fp32 values is exact there and cannot overflow, and HBM leaves the time for it.  No atomics.
-// The tensors are cut into tiles of at most BMT_CLIP_TILE elements by the caller's table, so a model of 200 tensors and one arena load the chip alike.
+// scales its tiles, walking them backwards: the tiles the norm read last are the ones the memory-side cache still holds.  The norm's loads are
+// ordinary ones for that reason; those and the stores of `apply` pass the caches by (nontemporal: 120 -> 97 us for 50 M fp32 values, 488 -> 424 us
+// for 335 M bf16 values into fp32; with nontemporal loads in the norm, too, 104 and 433 us).
+// Sums are 64-bit across a thread's share of a tile, and no value is lost to the range of fp32 (norm_tile).  No atomics.
+// The tensors are cut into tiles (of 32 KB: 8 loads of 16 bytes in flight per thread) by the caller's table, so a model of 200 tensors and one arena load the chip alike.
 #include "common.h"
 
 namespace {
@@ -19,18 +21,33 @@ static_assert(sizeof(Tile) == 24, "the caller packs tiles of 24 bytes");
 
 constexpr int CLIP_GRID = 2048;      // workgroups (and partial sums): 8 per CU
 
+// the table's pointers come out of memory: said to be global, they are not followed by flat accesses (which wait for LDS, too)
+template <typename T>
+using GlobalPtr = T __attribute__((address_space(1)))*;
+template <typename T>
+__device__ __forceinline__ GlobalPtr<T> global_at(const char* p, int64_t bytes) {
+    return (GlobalPtr<T>)(reinterpret_cast<uintptr_t>(p) + bytes);
+}
+
+template <int BYTES>
+struct Vec;
+template <>
+struct Vec<16> { typedef u32x4 T; };
+template <>
+struct Vec<8> { typedef u32x2 T; };
+
 template <int DT>
 constexpr int esize() { return DT == BMT_DT_F32 ? 4 : 2; }
 template <int DT>
 __device__ __forceinline__ float get1(const char* p) {
-    if constexpr (DT == BMT_DT_F32) return *reinterpret_cast<const float*>(p);
-    else if constexpr (DT == BMT_DT_BF16) return bf_bits2f(*reinterpret_cast<const uint16_t*>(p));
-    else return h_bits2f(*reinterpret_cast<const uint16_t*>(p));
+    if constexpr (DT == BMT_DT_F32) return *global_at<const float>(p, 0);
+    else if constexpr (DT == BMT_DT_BF16) return bf_bits2f(*global_at<const uint16_t>(p, 0));
+    else return h_bits2f(*global_at<const uint16_t>(p, 0));
 }
 template <int DT>
 __device__ __forceinline__ void put1(char* p, float x) {
-    if constexpr (DT == BMT_DT_F32) *reinterpret_cast<float*>(p) = x;
-    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)(pack_2<DT == BMT_DT_F16>(x, 0.f) & 0xffffu);
+    if constexpr (DT == BMT_DT_F32) *global_at<float>(p, 0) = x;
+    else *global_at<uint16_t>(p, 0) = (uint16_t)(pack_2<DT == BMT_DT_F16>(x, 0.f) & 0xffffu);
 }
 template <int DT>
 __device__ __forceinline__ void get16(const u32x4& v, float (&x)[16 / esize<DT>()]) {
@@ -46,11 +63,6 @@ struct Acc {
     double s;        // sum of squares
     uint32_t m;      // bits of max |g|: NaN compares above infinity
 };
-template <bool INF>
-__device__ __forceinline__ void add(Acc& a, float x) {
-    if constexpr (INF) a.m = max(a.m, __float_as_uint(x) & 0x7fffffffu);
-    else a.s = fma((double)x, (double)x, a.s);
-}
 
 // elements in front of the first 16-byte boundary
 template <int DT>
@@ -59,28 +71,50 @@ __device__ __forceinline__ int head_of(const char* p, int n) {
     return h < n ? h : n;
 }
 
-template <int DT, bool INF>
-__device__ __forceinline__ void norm_tile(const Tile& t, Acc& a) {
-    constexpr int E = esize<DT>(), G = 16 / E, U = 4;
+// A thread's share of a tile (at most 64 + 2 values).  Its squares are added in fp32 -- conversions and 64-bit products for every value took a third
+// of the time -- and that sum goes into the 64-bit one.  A sum outside [2^-80, 2^100] may have lost values to the ends of fp32's range (or is zero,
+// infinite or NaN): those shares, rare in gradients, are added again in 64 bits
+template <int DT, bool INF, bool WIDE>
+__device__ __forceinline__ void norm_share(const Tile& t, Acc& a, float& s32) {
+    constexpr int E = esize<DT>(), G = 16 / E, U = 8;
     const int h = head_of<DT>(t.g, t.n), nv = (t.n - h) / G, tail = h + nv * G;
-    const u32x4* v = reinterpret_cast<const u32x4*>(t.g + (int64_t)h * E);
+    const auto v = global_at<const u32x4>(t.g, (int64_t)h * E);
+    auto add = [&](float x) {
+        if constexpr (INF) a.m = max(a.m, __float_as_uint(x) & 0x7fffffffu);
+        else if constexpr (WIDE) a.s = fma((double)x, (double)x, a.s);
+        else s32 = __fmaf_rn(x, x, s32);
+    };
     for (int i = threadIdx.x; i < nv; i += 256 * U) {
         u32x4 q[U];
+        if (i + 256 * (U - 1) < nv) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            q[u] = u32x4{0, 0, 0, 0};
-            if (i + 256 * u < nv) q[u] = v[i + 256 * u];
+            for (int u = 0; u < U; ++u) q[u] = v[i + 256 * u];
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                q[u] = u32x4{0, 0, 0, 0};
+                if (i + 256 * u < nv) q[u] = v[i + 256 * u];
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float x[G];
             get16<DT>(q[u], x);
 #pragma unroll
-            for (int j = 0; j < G; ++j) add<INF>(a, x[j]);
+            for (int j = 0; j < G; ++j) add(x[j]);
         }
     }
-    if ((int)threadIdx.x < h) add<INF>(a, get1<DT>(t.g + threadIdx.x * E));
-    if ((int)threadIdx.x < t.n - tail) add<INF>(a, get1<DT>(t.g + (int64_t)(tail + threadIdx.x) * E));
+    if ((int)threadIdx.x < h) add(get1<DT>(t.g + threadIdx.x * E));
+    if ((int)threadIdx.x < t.n - tail) add(get1<DT>(t.g + (int64_t)(tail + threadIdx.x) * E));
+}
+template <int DT, bool INF>
+__device__ __forceinline__ void norm_tile(const Tile& t, Acc& a) {
+    float s32 = 0.f;
+    norm_share<DT, INF, false>(t, a, s32);
+    if constexpr (!INF) {
+        if (s32 >= 0x1p-80f && s32 <= 0x1p100f) a.s += (double)s32;
+        else norm_share<DT, INF, true>(t, a, s32);
+    }
 }
 
 template <bool INF>
@@ -102,8 +136,11 @@ template <bool INF>
 __global__ __launch_bounds__(256) void clip_norm_kernel(const Tile* __restrict__ tiles, int n, double* __restrict__ part) {
     __shared__ double red[4];
     Acc a = {0.0, 0u};
+    Tile next = {};
+    if ((int)blockIdx.x < n) next = tiles[blockIdx.x];
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
-        const Tile t = tiles[i];
+        const Tile t = next;
+        if (i + (int)gridDim.x < n) next = tiles[i + gridDim.x];      // (on its way beside this tile's data)
         const int dt = t.kind & 3;
         if (dt == BMT_DT_F32) norm_tile<BMT_DT_F32, INF>(t, a);
         else if (dt == BMT_DT_BF16) norm_tile<BMT_DT_BF16, INF>(t, a);
@@ -115,37 +152,40 @@ __global__ __launch_bounds__(256) void clip_norm_kernel(const Tile* __restrict__
 
 template <int DI, int DO>
 __device__ __forceinline__ void scale_tile(const Tile& t, float c) {
-    constexpr int EI = esize<DI>(), EO = esize<DO>(), G = 16 / EI, U = 4;
+    // the wider side in 16-byte accesses: 16-bit gradients into fp32 are loaded 8 bytes at a time
+    constexpr int EI = esize<DI>(), EO = esize<DO>(), G = 16 / (EI > EO ? EI : EO), U = 8;
+    typedef typename Vec<G * EI>::T TI;
+    typedef typename Vec<G * EO>::T TO;
     const int h = head_of<DI>(t.g, t.n);
-    if ((reinterpret_cast<uintptr_t>(t.out + (int64_t)h * EO) & (G * EO >= 16 ? 15 : 7)) != 0) {      // the two sides are not aligned alike
+    if ((reinterpret_cast<uintptr_t>(t.out + (int64_t)h * EO) & (G * EO - 1)) != 0) {      // the two sides are not aligned alike
         for (int i = threadIdx.x; i < t.n; i += 256) put1<DO>(t.out + (int64_t)i * EO, get1<DI>(t.g + (int64_t)i * EI) * c);
         return;
     }
     const int nv = (t.n - h) / G, tail = h + nv * G;
-    const u32x4* v = reinterpret_cast<const u32x4*>(t.g + (int64_t)h * EI);
-    char* o = t.out + (int64_t)h * EO;
+    const auto v = global_at<const TI>(t.g, (int64_t)h * EI);
+    const auto o = global_at<TO>(t.out, (int64_t)h * EO);
     for (int i = threadIdx.x; i < nv; i += 256 * U) {
-        u32x4 q[U];
+        TI q[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i + 256 * u < nv) q[u] = v[i + 256 * u];
+            if (i + 256 * u < nv) q[u] = __builtin_nontemporal_load(v + i + 256 * u);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i + 256 * u < nv) {
                 float x[G];
-                get16<DI>(q[u], x);
 #pragma unroll
-                for (int j = 0; j < G; ++j) x[j] *= c;
-                char* p = o + (int64_t)(i + 256 * u) * (G * EO);
-                if constexpr (DO == BMT_DT_F32) {
-#pragma unroll
-                    for (int k = 0; k < G / 4; ++k)
-                        reinterpret_cast<u32x4*>(p)[k] = u32x4{__float_as_uint(x[4 * k]), __float_as_uint(x[4 * k + 1]), __float_as_uint(x[4 * k + 2]), __float_as_uint(x[4 * k + 3])};
-                } else {
-#pragma unroll
-                    for (int k = 0; k < G / 4; ++k)
-                        reinterpret_cast<u32x2*>(p)[k] = u32x2{pack_2<DO == BMT_DT_F16>(x[4 * k], x[4 * k + 1]), pack_2<DO == BMT_DT_F16>(x[4 * k + 2], x[4 * k + 3])};
+                for (int j = 0; j < G; ++j) {
+                    if constexpr (DI == BMT_DT_F32) x[j] = __uint_as_float(q[u][j]) * c;
+                    else if constexpr (DI == BMT_DT_BF16) x[j] = bf_bits2f((q[u][j / 2] >> ((j & 1) * 16)) & 0xffffu) * c;
+                    else x[j] = h_bits2f((q[u][j / 2] >> ((j & 1) * 16)) & 0xffffu) * c;
                 }
+                TO w;
+#pragma unroll
+                for (int j = 0; j < G * EO / 4; ++j) {
+                    if constexpr (DO == BMT_DT_F32) w[j] = __float_as_uint(x[j]);
+                    else w[j] = pack_2<DO == BMT_DT_F16>(x[2 * j], x[2 * j + 1]);
+                }
+                __builtin_nontemporal_store(w, o + i + 256 * u);
             }
     }
     if ((int)threadIdx.x < h) put1<DO>(t.out + threadIdx.x * EO, get1<DI>(t.g + threadIdx.x * EI) * c);

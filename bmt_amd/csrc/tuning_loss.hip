@@ -96,6 +96,11 @@ struct Rows {
     int64_t mb, mt;
     int64_t pad;
 };
+struct Terms {      // what a policy row leaves for the sums: one 16-byte load
+    double loss;
+    float kl;
+    int flags;      // 1: the row counts, 2: the clip took its gradient
+};
 struct PolicyIn {
     const float *old, *ref, *adv;      // old NULL: the ratio is 1 (on-policy); ref NULL: no KL term
     int64_t ob, ot, rb, rt, ab, at;
@@ -109,37 +114,50 @@ __device__ __forceinline__ bool row_counts(const Rows& q, int b, int t, int64_t 
     return id != q.pad && (q.mask == nullptr || q.mask[b * q.mb + t * q.mt] != 0);
 }
 
-// the rows a mean divides by (those of sequence b, or all), as this thread's share of a group of NT
+// The rows a mean divides by (those of sequence b, or all of them; at most 2 NT), counted by the workgroup itself.  The loads are issued before the
+// row's own and used behind them: they come back while the row is on its way
 template <int NT>
-__device__ __forceinline__ int count_share(const Rows& q, const PolicyIn& p, int b) {
-    int n = 0;
-    if (p.counts || p.reduction == 0) return 0;
-    if (p.reduction == 2) {
-        for (int t = threadIdx.x; t < q.T; t += NT) n += row_counts(q, b, t, q.id[b * q.ib + t * q.it]);
-    } else {
-        for (int i = threadIdx.x; i < p.B * q.T; i += NT) n += row_counts(q, i / q.T, i % q.T, q.id[(i / q.T) * q.ib + (i % q.T) * q.it]);
+struct Counted {
+    int64_t id[2];
+    int on[2];
+    __device__ __forceinline__ void load(const Rows& q, const PolicyIn& p, int b) {
+        const int n = p.counts || p.reduction == 0 ? 0 : p.reduction == 2 ? q.T : p.B * q.T;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int i = threadIdx.x + NT * k;
+            id[k] = q.pad;
+            on[k] = 0;
+            if (i < n) {
+                const int bb = p.reduction == 2 ? b : i / q.T, t = p.reduction == 2 ? i : i % q.T;
+                id[k] = q.id[bb * q.ib + t * q.it];
+                on[k] = q.mask ? q.mask[bb * q.mb + t * q.mt] : 1;
+            }
+        }
     }
-    return n;
-}
+    __device__ __forceinline__ int share(const Rows& q) const { return (int)(id[0] != q.pad && on[0]) + (int)(id[1] != q.pad && on[1]); }
+};
 
 // A row as 16-byte granules of memory: the first one starts at or below the row's first element, so that vector accesses are aligned for every
 // start and every odd V; the elements of the two edge granules that are not the row's are never touched
 template <int DT>
 struct Row {
     using E = Elem<DT>;
-    char* base;      // 16-byte aligned
-    int phase, end;  // the row's elements are [phase, end) from base
+    const char* base;      // 16-byte aligned
+    int phase, end;        // the row's elements are [phase, end) from base
     __device__ __forceinline__ Row(const char* p, int V) {
-        const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-        base = reinterpret_cast<char*>(a & ~(uintptr_t)15);
-        phase = (int)(a & 15) / E::B;
+        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+        base = p - off;      // (no integer turned into a pointer: the compiler keeps seeing global memory)
+        phase = off / E::B;
         end = phase + V;
     }
     __device__ __forceinline__ int granules() const { return (end + E::G - 1) / E::G; }
     __device__ __forceinline__ bool inner(int k) const { return k * E::G >= phase && (k + 1) * E::G <= end; }
+    // LAST: nothing reads the row again, and the load passes the caches by, as the gradient's stores do (16 x 1024 x 32000 bf16 preference pass: 460 us
+    // without any of it, 441 with all loads like that, 416 with the forward pass's left to the caches, whose end the gradient kernel reads first)
+    template <bool LAST>
     __device__ __forceinline__ u32x4 load(int k) const {
         const char* p = base + (int64_t)k * 16;
-        if (inner(k)) return *reinterpret_cast<const u32x4*>(p);
+        if (inner(k)) return LAST ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)) : *reinterpret_cast<const u32x4*>(p);
         const uint32_t l = E::lowest();
         u32x4 v = {l, l, l, l};      // -inf: adds nothing to the maximum nor to the sum
 #pragma unroll
@@ -170,7 +188,7 @@ struct Row {
 // writes granule k of the row to `out` (same phase: 16-byte stores; another one: element by element)
 template <int DT>
 __device__ __forceinline__ void put_granule(const Row<DT>& row, int k, const u32x4& v, char* out, bool same) {
-    if (same && row.inner(k)) *reinterpret_cast<u32x4*>(out + ((int64_t)k * Elem<DT>::G - row.phase) * Elem<DT>::B) = v;
+    if (same && row.inner(k)) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out + ((int64_t)k * Elem<DT>::G - row.phase) * Elem<DT>::B));
     else row.store_elements(k, v, out);
 }
 __device__ __forceinline__ bool same_phase(const char* a, const char* b) { return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0; }
@@ -218,8 +236,8 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
 }
 
 // everything a policy row adds to the loss, in 64 bits: the differences of log-probabilities are small beside the values they come from, and the
-// KL term is second order in them.  Returns w_r; terms[0..2] = the row's share of the loss, its KL, whether the clip took its gradient
-__device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, int counted, double lp, double* terms) {
+// KL term is second order in them.  Returns w_r
+__device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, int counted, double lp, Terms* terms) {
     const double A = p.adv[b * p.ab + t * p.at];
     const double rho = p.old ? exp(lp - (double)p.old[b * p.ob + t * p.ot]) : exp(lp - lp);      // (lp - lp: NaN stays NaN)
     const double u = rho * A, c = fmin(fmax(rho, 1.0 - (double)p.lo), 1.0 + (double)p.hi) * A;
@@ -234,9 +252,7 @@ __device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, int
     double norm = 1.0;
     if (p.reduction == 1) norm = 1.0 / (double)max(p.counts ? p.counts[p.B] : counted, 1);
     else if (p.reduction == 2) norm = 1.0 / ((double)p.B * (double)max(p.counts ? p.counts[b] : counted, 1));
-    terms[0] = loss * norm;
-    terms[1] = kl;
-    terms[2] = clipped ? 1.0 : 0.0;
+    *terms = Terms{loss * norm, (float)kl, clipped ? 3 : 1};
     return (float)(w * norm);
 }
 
@@ -281,7 +297,7 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(Rows q, int B, int* __
 // One sweep with a running maximum and sum per thread.  stats[r] = {max, 1 / sum} for the gradient kernel (0, 0 where the row does not count).
 template <int DT, int NT, bool POLICY>
 __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float* __restrict__ logp, double* __restrict__ logp64, float2* __restrict__ stats, float* __restrict__ w,
-                                                        double* __restrict__ terms, int64_t rows) {
+                                                        Terms* __restrict__ terms) {
     using E = Elem<DT>;
     constexpr int U = 4;
     __shared__ float redf[NT / 64];
@@ -297,7 +313,7 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
             if (stats) stats[r] = make_float2(0.f, 0.f);
             if constexpr (POLICY) {
                 w[r] = 0.f;
-                terms[r] = terms[rows + r] = terms[2 * rows + r] = 0.0;
+                terms[r] = Terms{0.0, 0.f, 0};
             }
         }
         return;
@@ -305,6 +321,8 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
     const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
     const Row<DT> row(xr, q.V);
     const int n = row.granules();
+    Counted<NT> cnt;
+    if constexpr (POLICY) cnt.load(q, p, b);
     float xt = __builtin_nanf("");      // an id outside the vocabulary has no log-probability
     if (threadIdx.x == 0 && id >= 0 && id < q.V) xt = E::get1(xr + id * E::B);
     float m = -__builtin_huge_valf(), s = 0.f;
@@ -314,7 +332,7 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             v[i] = u32x4{l, l, l, l};
-            if (k0 + i * NT < n) v[i] = row.load(k0 + i * NT);
+            if (k0 + i * NT < n) v[i] = row.template load<false>(k0 + i * NT);
         }
         float x[U][E::G], bm = -__builtin_huge_valf();
 #pragma unroll
@@ -334,7 +352,7 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
         m = mn;
     }
     int counted = 0;
-    if constexpr (POLICY) counted = group_count<NT>(count_share<NT>(q, p, b), redi);
+    if constexpr (POLICY) counted = group_count<NT>(cnt.share(q), redi);
     const float M = group_max<NT>(m, redf);
     const double S = group_sum<NT>(m == -__builtin_huge_valf() ? (double)s : (double)s * (double)exp_neg_exact(m - M), redd);
     if (threadIdx.x == 0) {
@@ -343,20 +361,23 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
         if (logp64) logp64[r] = lp;
         if (stats) stats[r] = make_float2(M, (float)(1.0 / S));
         if constexpr (POLICY) {
-            double tr[3];
-            w[r] = policy_row(p, b, t, counted, lp, tr);
-            terms[r] = tr[0];
-            terms[rows + r] = tr[1];
-            terms[2 * rows + r] = tr[2];
+            w[r] = policy_row(p, b, t, counted, lp, &terms[r]);
         }
     }
+}
+
+// the granules as they were loaded, to be taken apart again: left alone the compiler keeps the floats of one use for the next (twice the registers)
+template <int NV>
+__device__ __forceinline__ void only_raw(u32x4 (&v)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i]));
 }
 
 // ---------------------------------------------------------------- policy loss: statistics, loss terms and gradient of a row in one visit
 // The row (at most NT * NV granules) stays in registers as it was loaded.
 template <int DT, int NT, int NV>
 __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, char* __restrict__ dx, int64_t db, int64_t dt, float* __restrict__ logp,
-                                                          float2* __restrict__ stats, float* __restrict__ w, double* __restrict__ terms, int64_t rows) {
+                                                          float2* __restrict__ stats, float* __restrict__ w, Terms* __restrict__ terms) {
     using E = Elem<DT>;
     __shared__ float redf[NT / 64];
     __shared__ double redd[NT / 64];
@@ -374,12 +395,14 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
             logp[r] = 0.f;
             stats[r] = make_float2(0.f, 0.f);
             w[r] = 0.f;
-            terms[r] = terms[rows + r] = terms[2 * rows + r] = 0.0;
+            terms[r] = Terms{0.0, 0.f, 0};
         }
         return;
     }
     const Row<DT> row(xr, q.V);
     const int n = row.granules();
+    Counted<NT> cnt;
+    cnt.load(q, p, b);
     float xt = __builtin_nanf("");      // an id outside the vocabulary has no log-probability
     if (threadIdx.x == 0 && id >= 0 && id < q.V) xt = E::get1(xr + id * E::B);
     u32x4 v[NV];
@@ -387,7 +410,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         v[i] = u32x4{l, l, l, l};
-        if ((int)threadIdx.x + NT * i < n) v[i] = row.load(threadIdx.x + NT * i);
+        if ((int)threadIdx.x + NT * i < n) v[i] = row.template load<true>(threadIdx.x + NT * i);
     }
     float m = -__builtin_huge_valf();
 #pragma unroll
@@ -397,8 +420,9 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
 #pragma unroll
         for (int j = 0; j < E::G; ++j) m = fmaxf(m, x[j]);
     }
-    const int counted = group_count<NT>(count_share<NT>(q, p, b), redi);
+    const int counted = group_count<NT>(cnt.share(q), redi);
     m = group_max<NT>(m, redf);
+    only_raw(v);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -411,19 +435,16 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
         }
     }
     const double S = group_sum<NT>((double)s, redd);
+    only_raw(v);
     if (threadIdx.x == 0) {
         const double lp = ((double)xt - (double)m) - log(S);
-        double tr[3];
-        const float wr = policy_row(p, b, t, counted, lp, tr);
+        const float wr = policy_row(p, b, t, counted, lp, &terms[r]);
         const float is = (float)(1.0 / S);
         wc[0] = wr;
         wc[1] = is;
         logp[r] = (float)lp;
         stats[r] = make_float2(m, is);
         w[r] = wr;
-        terms[r] = tr[0];
-        terms[rows + r] = tr[1];
-        terms[2 * rows + r] = tr[2];
     }
     __syncthreads();
     const float wr = wc[0], c = -wr * wc[1];
@@ -448,15 +469,24 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
 }
 
 // loss[0] = sum of the rows' shares, info[0] = mean KL, info[1] = share of rows whose gradient the clip took (means over the rows that count)
-__global__ __launch_bounds__(1024) void policy_finish_kernel(const double* __restrict__ terms, const float2* __restrict__ stats, int64_t rows, float* __restrict__ loss,
+__global__ __launch_bounds__(1024) void policy_finish_kernel(const Terms* __restrict__ terms, int64_t rows, float* __restrict__ loss,
                                                               float* __restrict__ info) {
     __shared__ double red[4][16];
     double a[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    for (int64_t r0 = threadIdx.x; r0 < rows; r0 += 8 * 1024) {      // 8 records on their way at a time
+        Terms t[8];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) a[k] += terms[k * rows + r];
-        a[3] += stats[r].y == 0.f ? 0.0 : 1.0;      // (a row that counts has a finite sum)
+        for (int i = 0; i < 8; ++i) {
+            t[i] = Terms{0.0, 0.f, 0};
+            if (r0 + 1024 * i < rows) t[i] = terms[r0 + 1024 * i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            a[0] += t[i].loss;
+            a[1] += (double)t[i].kl;
+            a[2] += t[i].flags >> 1;
+            a[3] += t[i].flags & 1;
+        }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -502,7 +532,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
         const bool same = same_phase(xr, dr);
         for (int k = threadIdx.x; k < n; k += NT) {
             float x[E::G];
-            E::get(row.load(k), x);
+            E::get(row.template load<true>(k), x);
 #pragma unroll
             for (int j = 0; j < E::G; ++j) x[j] = exp_neg(x[j] - m) * c;
             if (k == kt) {
@@ -595,14 +625,16 @@ inline int threads_for(int64_t rows, int64_t granules) {
     return rows < 512 && granules > 1024 ? 1024 : 256;
 }
 
+inline int64_t granules_of(int V, int dtype) { return ((int64_t)V * elem_bytes(dtype) + 15) / 16; }
+
 template <int DT>
-void launch_logp(const Rows& q, const PolicyIn* p, float* logp, double* logp64, float2* stats, float* w, double* terms, int64_t rows, hipStream_t st) {
-    const int nt = threads_for(rows, ((int64_t)q.V + Elem<DT>::G - 1) / Elem<DT>::G);
+void launch_logp(const Rows& q, const PolicyIn* p, float* logp, double* logp64, float2* stats, float* w, Terms* terms, int64_t rows, hipStream_t st) {
+    const int nt = threads_for(rows, granules_of(q.V, DT));
     const PolicyIn none = {};
 #define BMT_ROWS(NT)                                                                                                                               \
     do {                                                                                                                                           \
-        if (p) hipLaunchKernelGGL((logp_rows_kernel<DT, NT, true>), dim3((unsigned)rows), dim3(NT), 0, st, q, *p, logp, logp64, stats, w, terms, rows);      \
-        else hipLaunchKernelGGL((logp_rows_kernel<DT, NT, false>), dim3((unsigned)rows), dim3(NT), 0, st, q, none, logp, logp64, stats, w, terms, rows);     \
+        if (p) hipLaunchKernelGGL((logp_rows_kernel<DT, NT, true>), dim3((unsigned)rows), dim3(NT), 0, st, q, *p, logp, logp64, stats, w, terms);      \
+        else hipLaunchKernelGGL((logp_rows_kernel<DT, NT, false>), dim3((unsigned)rows), dim3(NT), 0, st, q, none, logp, logp64, stats, w, terms);     \
     } while (0)
     if (nt == 64) BMT_ROWS(64);
     else if (nt == 256) BMT_ROWS(256);
@@ -613,7 +645,7 @@ void launch_logp(const Rows& q, const PolicyIn* p, float* logp, double* logp64, 
 template <int DT>
 void launch_grad(const Rows& q, const float2* stats, const float* w, int64_t wb, int64_t wt, const float* g, int once, void* dx, int64_t db, int64_t dt, int64_t rows,
                  hipStream_t st) {
-    const int nt = threads_for(rows, ((int64_t)q.V + Elem<DT>::G - 1) / Elem<DT>::G);
+    const int nt = threads_for(rows, granules_of(q.V, DT));
     const unsigned grid = (unsigned)(once && rows > 2048 ? 2048 : rows);      // (once: usually every workgroup ends at its first instruction)
 #define BMT_GRAD(NT) hipLaunchKernelGGL((logit_grad_kernel<DT, NT>), dim3(grid), dim3(NT), 0, st, q, stats, w, wb, wt, g, once, (char*)dx, db, dt, rows)
     if (nt == 64) BMT_GRAD(64);
@@ -624,11 +656,11 @@ void launch_grad(const Rows& q, const float2* stats, const float* w, int64_t wb,
 
 // the fused form where a row fits the registers of a workgroup; false: it does not
 template <int DT>
-bool launch_policy(const Rows& q, const PolicyIn& p, void* dx, int64_t db, int64_t dt, float* logp, float2* stats, float* w, double* terms, int64_t rows, hipStream_t st) {
-    const int64_t n = ((int64_t)q.V + Elem<DT>::G - 1) / Elem<DT>::G + 1;      // (+ 1: a row that starts inside a granule)
+bool launch_policy(const Rows& q, const PolicyIn& p, void* dx, int64_t db, int64_t dt, float* logp, float2* stats, float* w, Terms* terms, int64_t rows, hipStream_t st) {
+    const int64_t n = granules_of(q.V, DT) + 1;      // (+ 1: a row that starts inside a granule)
 #define BMT_POL(NT, NV)                                                                                                                                       \
     do {                                                                                                                                                      \
-        hipLaunchKernelGGL((policy_rows_kernel<DT, NT, NV>), dim3((unsigned)rows), dim3(NT), 0, st, q, p, (char*)dx, db, dt, logp, stats, w, terms, rows);     \
+        hipLaunchKernelGGL((policy_rows_kernel<DT, NT, NV>), dim3((unsigned)rows), dim3(NT), 0, st, q, p, (char*)dx, db, dt, logp, stats, w, terms);     \
         return true;                                                                                                                                          \
     } while (0)
     const int nt = threads_for(rows, n - 1);
@@ -688,7 +720,7 @@ extern "C" int bmt_logit_grad(const void* logits, int dtype, int64_t sb, int64_t
 
 extern "C" int64_t bmt_policy_ws_bytes(int B, int T) {
     if (B < 0 || T < 0) return 0;
-    return (int64_t)B * T * (3 * 8 + 3 * 4) + ((int64_t)B + 1) * 4;
+    return (int64_t)B * T * (16 + 8 + 4) + ((int64_t)B + 1) * 4;
 }
 
 extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
@@ -702,20 +734,21 @@ extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_
     BMT_CHECK_ARG(adv && loss && info && logp && ws, "bmt_policy_loss: null pointer");
     BMT_CHECK_ARG(reduction >= 0 && reduction <= 2, "bmt_policy_loss: unknown reduction %d", reduction);
     BMT_CHECK_ARG(clip_low >= 0.f && clip_high >= 0.f, "bmt_policy_loss: negative clip range");
-    BMT_CHECK_ARG(ws_bytes >= bmt_policy_ws_bytes(B, T) && (reinterpret_cast<uintptr_t>(ws) & 7) == 0, "bmt_policy_loss: workspace of %lld bytes is too small or not aligned",
+    BMT_CHECK_ARG(ws_bytes >= bmt_policy_ws_bytes(B, T) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0, "bmt_policy_loss: workspace of %lld bytes is too small or not aligned",
                   (long long)ws_bytes);
     BMT_CHECK_ARG(!dlogits || (db >= 0 && dt >= 0 && (reinterpret_cast<uintptr_t>(dlogits) & (elem_bytes(dtype) - 1)) == 0), "bmt_policy_loss: bad gradient layout");
     hipStream_t s = (hipStream_t)stream;
-    // workspace: terms [3][rows] (64-bit) | stats [rows][2] | w [rows] | counts [B + 1]
-    double* terms = (double*)ws;
-    float2* stats = (float2*)(terms + 3 * rows);
+    // workspace: terms [rows] | stats [rows][2] | w [rows] | counts [B + 1]
+    Terms* terms = (Terms*)ws;
+    float2* stats = (float2*)(terms + rows);
     float* w = (float*)(stats + rows);
     int* counts = (int*)(w + rows);
-    // what a mean divides by: a few thousand ids are counted by every row's workgroup beside its loads (a launch less), more by one of their own
+    // what a mean divides by: two ids per thread are counted by every row's workgroup beside its loads (a launch less), more by one of their own
     const int64_t divides = reduction == 0 ? 0 : reduction == 1 ? rows : T;
+    const bool count = divides > 2 * threads_for(rows, granules_of(V, dtype));
     const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
-    const PolicyIn p = {old_logp, ref_logp, adv, ob, ot, rb, rt, ab, at, clip_low, clip_high, kl_coef, reduction, B, divides > 2048 ? counts : nullptr};
-    if (divides > 2048) hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, s, q, B, counts);
+    const PolicyIn p = {old_logp, ref_logp, adv, ob, ot, rb, rt, ab, at, clip_low, clip_high, kl_coef, reduction, B, count ? counts : nullptr};
+    if (count) hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, s, q, B, counts);
     bool done = false;
 #define BMT_CALL(DT) done = launch_policy<DT>(q, p, dlogits, db, dt, logp, stats, w, terms, rows, s)
     if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
@@ -728,7 +761,7 @@ extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_
         if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
 #undef BMT_CALL
     }
-    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, s, terms, stats, rows, loss, info);
+    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, s, terms, rows, loss, info);
     BMT_CHECK_LAUNCH("bmt_policy_loss");
     return BMT_OK;
 }

@@ -138,7 +138,7 @@ def clip_grad_norm_(parameters: Iterable[torch.nn.Parameter], max_norm: float) -
     return sq.sqrt().squeeze(0)
 
 
-CLIP_TILE = 8192        # elements per tile of GradClipper's table: 32 per thread of a workgroup
+CLIP_TILE = 32768       # bytes of gradient per tile of GradClipper's table: 128 per thread of a workgroup
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -214,10 +214,11 @@ class GradClipper:
         assert entry.itemsize == lib.bmt_clip_tile_bytes()
         rows = []
         for g, o, pg, po in zip(self.grads, self.out, *self._ptrs):
-            first = np.arange(0, g.numel(), CLIP_TILE, dtype=np.uint64)
+            tile = CLIP_TILE // g.element_size()
+            first = np.arange(0, g.numel(), tile, dtype=np.uint64)
             r = np.empty(len(first), entry)
             r["g"], r["out"] = pg + first * np.uint64(g.element_size()), po + first * np.uint64(o.element_size())
-            r["n"] = np.minimum(CLIP_TILE, g.numel() - first.astype(np.int64))
+            r["n"] = np.minimum(tile, g.numel() - first.astype(np.int64))
             r["kind"] = _DTYPES[g.dtype] | _DTYPES[o.dtype] << 2
             rows.append(r)
         rows = np.concatenate(rows)
