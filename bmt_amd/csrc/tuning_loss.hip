@@ -107,34 +107,55 @@ struct PolicyIn {
     float lo, hi, beta;
     int reduction;                     // 0 sum, 1 mean over the rows that count, 2 mean over sequences of their means
     int B;
-    const int* counts;                 // [B] rows that count per sequence, [B] their total; NULL: every workgroup counts what it needs
+    const int* counts;                 // what count_rows_kernel counted (per sequence, or n_counts parts of all); NULL: every workgroup counts itself
+    int n_counts;
 };
+constexpr int COUNT_PARTS = 256, FINISH_PARTS = 64;      // most workgroups of the counting and of the adding kernels
 
 __device__ __forceinline__ bool row_counts(const Rows& q, int b, int t, int64_t id) {
     return id != q.pad && (q.mask == nullptr || q.mask[b * q.mb + t * q.mt] != 0);
 }
 
-// The rows a mean divides by (those of sequence b, or all of them; at most 2 NT), counted by the workgroup itself.  The loads are issued before the
-// row's own and used behind them: they come back while the row is on its way
+// The rows a mean divides by (those of sequence b, or all of them): few are counted by the workgroup itself, of many it adds up the parts.  The
+// loads are issued before the row's own and used behind them: they come back while the row is on its way
 template <int NT>
 struct Counted {
-    int64_t id[2];
-    int on[2];
+    static constexpr int K = NT == 64 ? 4 : 2;      // ids per thread: COUNT_PARTS numbers, too
+    int64_t id[K];
+    int on[K];
     __device__ __forceinline__ void load(const Rows& q, const PolicyIn& p, int b) {
-        const int n = p.counts || p.reduction == 0 ? 0 : p.reduction == 2 ? q.T : p.B * q.T;
+        const int n = p.reduction == 0 ? 0 : p.counts ? (p.reduction == 2 ? 1 : p.n_counts) : p.reduction == 2 ? q.T : p.B * q.T;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < K; ++k) {
             const int i = threadIdx.x + NT * k;
             id[k] = q.pad;
             on[k] = 0;
             if (i < n) {
-                const int bb = p.reduction == 2 ? b : i / q.T, t = p.reduction == 2 ? i : i % q.T;
-                id[k] = q.id[bb * q.ib + t * q.it];
-                on[k] = q.mask ? q.mask[bb * q.mb + t * q.mt] : 1;
+                if (p.counts) on[k] = p.counts[p.reduction == 2 ? b : i];
+                else {
+                    const int bb = p.reduction == 2 ? b : i / q.T, t = p.reduction == 2 ? i : i % q.T;
+                    id[k] = q.id[bb * q.ib + t * q.it];
+                    on[k] = q.mask ? q.mask[bb * q.mb + t * q.mt] : 1;
+                }
             }
         }
     }
-    __device__ __forceinline__ int share(const Rows& q) const { return (int)(id[0] != q.pad && on[0]) + (int)(id[1] != q.pad && on[1]); }
+    __device__ __forceinline__ int share(const Rows& q, const PolicyIn& p) const {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) n += p.counts ? on[k] : (int)(id[k] != q.pad && on[k]);
+        return n;
+    }
+};
+
+// a policy row's own numbers, on their way beside the row
+struct RowIn {
+    float adv, old, ref;
+    __device__ __forceinline__ void load(const PolicyIn& p, int b, int t) {
+        adv = p.adv[b * p.ab + t * p.at];
+        old = p.old ? p.old[b * p.ob + t * p.ot] : 0.f;
+        ref = p.ref ? p.ref[b * p.rb + t * p.rt] : 0.f;
+    }
 };
 
 // A row as 16-byte granules of memory: the first one starts at or below the row's first element, so that vector accesses are aligned for every
@@ -235,62 +256,72 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
     return s;
 }
 
+// e^d - 1 - d.  Policies that are compared lie close together: up to 1/2 by its series (15 terms: below 1e-16 of it), without cancellation and without
+// the library's exponential, which is long for the one thread that works while the workgroup waits
+__device__ __forceinline__ double exp_rest(double d) {
+    if (!(fabs(d) <= 0.5)) return exp(d) - 1.0 - d;      // (NaN goes this way)
+    double s = 1.0;
+#pragma unroll
+    for (int k = 15; k > 2; --k) s = fma(s * d, 1.0 / k, 1.0);
+    return 0.5 * d * d * s;
+}
+
+// 1 / what a row's loss is divided by
+__device__ __forceinline__ double row_norm(const PolicyIn& p, int counted) {
+    return p.reduction == 0 ? 1.0 : 1.0 / ((p.reduction == 2 ? (double)p.B : 1.0) * (double)max(counted, 1));
+}
+
 // everything a policy row adds to the loss, in 64 bits: the differences of log-probabilities are small beside the values they come from, and the
 // KL term is second order in them.  Returns w_r
-__device__ __forceinline__ float policy_row(const PolicyIn& p, int b, int t, int counted, double lp, Terms* terms) {
-    const double A = p.adv[b * p.ab + t * p.at];
-    const double rho = p.old ? exp(lp - (double)p.old[b * p.ob + t * p.ot]) : exp(lp - lp);      // (lp - lp: NaN stays NaN)
+__device__ __forceinline__ float policy_row(const PolicyIn& p, const RowIn& in, double norm, double lp, Terms* terms) {
+    const double A = in.adv, dold = lp - (p.old ? (double)in.old : lp);      // (lp - lp: NaN stays NaN)
+    const double rho = fabs(dold) <= 0.5 ? 1.0 + dold + exp_rest(dold) : exp(dold);      // (a token of probability 0 now: 0)
     const double u = rho * A, c = fmin(fmax(rho, 1.0 - (double)p.lo), 1.0 + (double)p.hi) * A;
     const bool clipped = u > c;
     double loss = clipped ? -c : -u, w = clipped ? 0.0 : -u, kl = 0.0;
     if (p.ref) {
-        const double d = (double)p.ref[b * p.rb + t * p.rt] - lp, em = expm1(d);
-        kl = em - d;
+        const double d = (double)in.ref - lp;
+        kl = exp_rest(d);
         loss += (double)p.beta * kl;
-        w -= (double)p.beta * em;
+        w -= (double)p.beta * (kl + d);
     }
-    double norm = 1.0;
-    if (p.reduction == 1) norm = 1.0 / (double)max(p.counts ? p.counts[p.B] : counted, 1);
-    else if (p.reduction == 2) norm = 1.0 / ((double)p.B * (double)max(p.counts ? p.counts[b] : counted, 1));
     *terms = Terms{loss * norm, (float)kl, clipped ? 3 : 1};
     return (float)(w * norm);
 }
 
-// ---------------------------------------------------------------- rows that count, per sequence and in all (one workgroup)
-// a wave per sequence, or -- short sequences -- a thread per sequence: 64 lanes would wait on a handful of loads
-__global__ __launch_bounds__(1024) void count_rows_kernel(Rows q, int B, int* __restrict__ counts) {
-    __shared__ int red[16];
-    int total = 0;
-    if (q.T < 32) {
-        for (int b = threadIdx.x; b < B; b += 1024) {
-            int n = 0;
-            for (int t = 0; t < q.T; ++t) n += row_counts(q, b, t, q.id[b * q.ib + t * q.it]);
-            counts[b] = n;
-            total += n;
-        }
-    } else {
-        for (int b = threadIdx.x >> 6; b < B; b += 16) {
-            int n = 0;
+// ---------------------------------------------------------------- rows that count: counts[b] (a wave per sequence) or parts of all rows
+__global__ __launch_bounds__(256) void count_rows_kernel(Rows q, int B, int per_sequence, int64_t rows, int* __restrict__ counts) {
+    __shared__ int red[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int n = 0;
+    if (per_sequence) {
+        const int b = blockIdx.x * 4 + wave;
+        if (b < B) {
 #pragma unroll 4
-            for (int t = threadIdx.x & 63; t < q.T; t += 64) {
+            for (int t = lane; t < q.T; t += 64) {
                 const int64_t id = q.id[b * q.ib + t * q.it];
                 const int on = q.mask ? q.mask[b * q.mb + t * q.mt] : 1;
                 n += (id != q.pad) & (on != 0);
             }
-            total += n;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-            if ((threadIdx.x & 63) == 0) counts[b] = n;
+        }
+    } else {
+#pragma unroll 4
+        for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < rows; r += (int64_t)gridDim.x * 256) {
+            const int b = (int)(r / q.T), t = (int)(r % q.T);
+            const int64_t id = q.id[b * q.ib + t * q.it];
+            const int on = q.mask ? q.mask[b * q.mb + t * q.mt] : 1;
+            n += (id != q.pad) & (on != 0);
         }
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = total;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 16; ++i) total += red[i];
-        counts[B] = total;
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    if (per_sequence) {
+        if (lane == 0 && (int)blockIdx.x * 4 + wave < B) counts[blockIdx.x * 4 + wave] = n;
+        return;
     }
+    if (lane == 0) red[wave] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
 // ---------------------------------------------------------------- forward: statistics and log-probability of every row, any V
@@ -322,7 +353,11 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
     const Row<DT> row(xr, q.V);
     const int n = row.granules();
     Counted<NT> cnt;
-    if constexpr (POLICY) cnt.load(q, p, b);
+    RowIn in = {};
+    if constexpr (POLICY) {
+        cnt.load(q, p, b);
+        if (threadIdx.x == 0) in.load(p, b, t);
+    }
     float xt = __builtin_nanf("");      // an id outside the vocabulary has no log-probability
     if (threadIdx.x == 0 && id >= 0 && id < q.V) xt = E::get1(xr + id * E::B);
     float m = -__builtin_huge_valf(), s = 0.f;
@@ -351,8 +386,8 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
         s += a;
         m = mn;
     }
-    int counted = 0;
-    if constexpr (POLICY) counted = group_count<NT>(cnt.share(q), redi);
+    double norm = 1.0;
+    if constexpr (POLICY) norm = row_norm(p, group_count<NT>(cnt.share(q, p), redi));
     const float M = group_max<NT>(m, redf);
     const double S = group_sum<NT>(m == -__builtin_huge_valf() ? (double)s : (double)s * (double)exp_neg_exact(m - M), redd);
     if (threadIdx.x == 0) {
@@ -361,7 +396,7 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
         if (logp64) logp64[r] = lp;
         if (stats) stats[r] = make_float2(M, (float)(1.0 / S));
         if constexpr (POLICY) {
-            w[r] = policy_row(p, b, t, counted, lp, &terms[r]);
+            w[r] = policy_row(p, in, norm, lp, &terms[r]);
         }
     }
 }
@@ -402,7 +437,9 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     const Row<DT> row(xr, q.V);
     const int n = row.granules();
     Counted<NT> cnt;
+    RowIn in = {};
     cnt.load(q, p, b);
+    if (threadIdx.x == 0) in.load(p, b, t);
     float xt = __builtin_nanf("");      // an id outside the vocabulary has no log-probability
     if (threadIdx.x == 0 && id >= 0 && id < q.V) xt = E::get1(xr + id * E::B);
     u32x4 v[NV];
@@ -420,7 +457,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
 #pragma unroll
         for (int j = 0; j < E::G; ++j) m = fmaxf(m, x[j]);
     }
-    const int counted = group_count<NT>(cnt.share(q), redi);
+    const double norm = row_norm(p, group_count<NT>(cnt.share(q, p), redi));
     m = group_max<NT>(m, redf);
     only_raw(v);
     float s = 0.f;
@@ -438,7 +475,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     only_raw(v);
     if (threadIdx.x == 0) {
         const double lp = ((double)xt - (double)m) - log(S);
-        const float wr = policy_row(p, b, t, counted, lp, &terms[r]);
+        const float wr = policy_row(p, in, norm, lp, &terms[r]);
         const float is = (float)(1.0 / S);
         wc[0] = wr;
         wc[1] = is;
@@ -450,9 +487,11 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     const float wr = wc[0], c = -wr * wc[1];
     const int kt = (int)((row.phase + id) / E::G), jt = (int)((row.phase + id) % E::G);      // (outside the vocabulary: wr is NaN everywhere)
     const bool same = same_phase(xr, dr);
+    int k0 = threadIdx.x;
+    asm volatile("" : "+v"(k0));      // (the places of the stores are worked out anew, not kept from the loads: two registers per granule)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int k = threadIdx.x + NT * i;
+        const int k = k0 + NT * i;
         if (k < n) {
             float x[E::G];
             E::get(v[i], x);
@@ -468,24 +507,31 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     }
 }
 
-// loss[0] = sum of the rows' shares, info[0] = mean KL, info[1] = share of rows whose gradient the clip took (means over the rows that count)
-__global__ __launch_bounds__(1024) void policy_finish_kernel(const Terms* __restrict__ terms, int64_t rows, float* __restrict__ loss,
+// loss[0] = sum of the rows' shares, info[0] = mean KL, info[1] = share of rows whose gradient the clip took (means over the rows that count).
+// One workgroup, or -- many rows -- one that adds the sums of several (part: 4 numbers each)
+__global__ __launch_bounds__(1024) void policy_finish_kernel(const Terms* __restrict__ terms, int64_t rows, double* __restrict__ part, int parts, float* __restrict__ loss,
                                                               float* __restrict__ info) {
     __shared__ double red[4][16];
     double a[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int64_t r0 = threadIdx.x; r0 < rows; r0 += 8 * 1024) {      // 8 records on their way at a time
-        Terms t[8];
+    if (parts > 0) {
+        if ((int)threadIdx.x < parts)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            t[i] = Terms{0.0, 0.f, 0};
-            if (r0 + 1024 * i < rows) t[i] = terms[r0 + 1024 * i];
-        }
+            for (int k = 0; k < 4; ++k) a[k] = part[4 * threadIdx.x + k];
+    } else {
+        for (int64_t r0 = (int64_t)blockIdx.x * 8192 + threadIdx.x; r0 < rows; r0 += (int64_t)gridDim.x * 8192) {      // 8 records on their way at a time
+            Terms t[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            a[0] += t[i].loss;
-            a[1] += (double)t[i].kl;
-            a[2] += t[i].flags >> 1;
-            a[3] += t[i].flags & 1;
+            for (int i = 0; i < 8; ++i) {
+                t[i] = Terms{0.0, 0.f, 0};
+                if (r0 + 1024 * i < rows) t[i] = terms[r0 + 1024 * i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[0] += t[i].loss;
+                a[1] += (double)t[i].kl;
+                a[2] += t[i].flags >> 1;
+                a[3] += t[i].flags & 1;
+            }
         }
     }
 #pragma unroll
@@ -494,14 +540,15 @@ __global__ __launch_bounds__(1024) void policy_finish_kernel(const Terms* __rest
         if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = a[k];
     }
     __syncthreads();
-    if (threadIdx.x < 3) {
+    if (threadIdx.x < 4) {
         double v = 0.0, n = 0.0;
         for (int i = 0; i < 16; ++i) {
             v += red[threadIdx.x][i];
             n += red[3][i];
         }
-        if (threadIdx.x == 0) loss[0] = (float)v;
-        else info[threadIdx.x - 1] = (float)(v / fmax(n, 1.0));
+        if (gridDim.x > 1) part[4 * blockIdx.x + threadIdx.x] = v;
+        else if (threadIdx.x == 0) loss[0] = (float)v;
+        else if (threadIdx.x < 3) info[threadIdx.x - 1] = (float)(v / fmax(n, 1.0));
     }
 }
 
@@ -670,6 +717,7 @@ bool launch_policy(const Rows& q, const PolicyIn& p, void* dx, int64_t db, int64
     if (nt == 256 && n <= 256 * 8) BMT_POL(256, 8);
     if (nt == 256 && n <= 256 * 12) BMT_POL(256, 12);
     if (nt == 256 && n <= 256 * 16) BMT_POL(256, 16);
+    if (nt == 256 && n <= 512 * 16) BMT_POL(512, 16);
     if (n <= 1024 * 4) BMT_POL(1024, 4);
     if (n <= 1024 * 8) BMT_POL(1024, 8);
     if (n <= 1024 * 16) BMT_POL(1024, 16);
@@ -720,7 +768,7 @@ extern "C" int bmt_logit_grad(const void* logits, int dtype, int64_t sb, int64_t
 
 extern "C" int64_t bmt_policy_ws_bytes(int B, int T) {
     if (B < 0 || T < 0) return 0;
-    return (int64_t)B * T * (16 + 8 + 4) + ((int64_t)B + 1) * 4;
+    return FINISH_PARTS * 32 + (int64_t)B * T * (16 + 8 + 4) + (int64_t)(B > COUNT_PARTS ? B : COUNT_PARTS) * 4;
 }
 
 extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* ids, int64_t ib, int64_t it,
@@ -738,17 +786,20 @@ extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_
                   (long long)ws_bytes);
     BMT_CHECK_ARG(!dlogits || (db >= 0 && dt >= 0 && (reinterpret_cast<uintptr_t>(dlogits) & (elem_bytes(dtype) - 1)) == 0), "bmt_policy_loss: bad gradient layout");
     hipStream_t s = (hipStream_t)stream;
-    // workspace: terms [rows] | stats [rows][2] | w [rows] | counts [B + 1]
-    Terms* terms = (Terms*)ws;
+    // workspace: sums of the adding kernel | terms [rows] | stats [rows][2] | w [rows] | counts
+    double* part = (double*)ws;
+    Terms* terms = (Terms*)(part + 4 * FINISH_PARTS);
     float2* stats = (float2*)(terms + rows);
     float* w = (float*)(stats + rows);
     int* counts = (int*)(w + rows);
-    // what a mean divides by: two ids per thread are counted by every row's workgroup beside its loads (a launch less), more by one of their own
+    // what a mean divides by: a few ids per thread are counted by every row's workgroup beside its loads (a launch less), more by one of their own
     const int64_t divides = reduction == 0 ? 0 : reduction == 1 ? rows : T;
-    const bool count = divides > 2 * threads_for(rows, granules_of(V, dtype));
+    const int nt = threads_for(rows, granules_of(V, dtype));
+    const bool count = divides > (nt == 64 ? 4 : 2) * nt;
+    const int parts = reduction == 2 ? bmt_cdiv(B, 4) : (int)(rows > 1024 * COUNT_PARTS ? COUNT_PARTS : (rows + 1023) / 1024);
     const Rows q = {(const char*)logits, sb, st, T, V, ids, ib, it, mask, mb, mt, pad_idx};
-    const PolicyIn p = {old_logp, ref_logp, adv, ob, ot, rb, rt, ab, at, clip_low, clip_high, kl_coef, reduction, B, count ? counts : nullptr};
-    if (count) hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, s, q, B, counts);
+    const PolicyIn p = {old_logp, ref_logp, adv, ob, ot, rb, rt, ab, at, clip_low, clip_high, kl_coef, reduction, B, count ? counts : nullptr, parts};
+    if (count) hipLaunchKernelGGL(count_rows_kernel, dim3(parts), dim3(256), 0, s, q, B, (int)(reduction == 2), rows, counts);
     bool done = false;
 #define BMT_CALL(DT) done = launch_policy<DT>(q, p, dlogits, db, dt, logp, stats, w, terms, rows, s)
     if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
@@ -761,7 +812,10 @@ extern "C" int bmt_policy_loss(const void* logits, int dtype, int64_t sb, int64_
         if (dlogits) BMT_BY_DTYPE(dtype, BMT_CALL);
 #undef BMT_CALL
     }
-    hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, s, terms, rows, loss, info);
+    // (8192 rows a workgroup: one batch of loads per thread)
+    const int wgs = rows <= 16384 ? 1 : (int)((rows + 8191) / 8192 < FINISH_PARTS ? (rows + 8191) / 8192 : FINISH_PARTS);
+    hipLaunchKernelGGL(policy_finish_kernel, dim3(wgs), dim3(1024), 0, s, terms, rows, part, 0, loss, info);
+    if (wgs > 1) hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, s, terms, rows, part, wgs, loss, info);
     BMT_CHECK_LAUNCH("bmt_policy_loss");
     return BMT_OK;
 }

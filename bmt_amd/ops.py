@@ -3784,7 +3784,7 @@ class PolicyLossFn(torch.autograd.Function):
         x, ids, mask, ws = ctx.saved_tensors
         rows = x.shape[0] * x.shape[1]
         out, ctx.dlogits = ctx.dlogits, None      # (a second backward pass through a kept graph computes its own)
-        d = _logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr() + 16 * rows, ws.data_ptr() + 24 * rows, x.shape[1], 1, g, out)
+        d = _logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr() + 2048 + 16 * rows, ws.data_ptr() + 2048 + 24 * rows, x.shape[1], 1, g, out)
         return (d,) + (None,) * 10
 
 

@@ -639,7 +639,7 @@ int bmt_loss_finish(const float* kl, const int64_t* n_tokens, float* loss, float
  *                        1: mean over the rows that count, 2: mean over the B sequences of their means (0 where nothing counts).
  *                        loss[0]; info[0] = mean KL, info[1] = share of rows whose policy gradient the clip took; logp [B * T].  dlogits
  *                        (optional): the gradient of loss, in the same pass.  ws: bmt_policy_ws_bytes, 16-byte aligned; it keeps what
- *                        bmt_logit_grad wants: stats at 16 * B * T bytes, w (wb = T, wt = 1) at 24 * B * T bytes
+ *                        bmt_logit_grad wants: stats at 2048 + 16 * B * T bytes, w (wb = T, wt = 1) at 2048 + 24 * B * T
  *   bmt_preference_loss  sequences b and b + B / 2 are a pair (preferred, rejected): S_b = sum of logp over the rows that count (mean_logp: their
  *                        mean), rewards[b] = beta (S_b - ref_logp[b * ref_stride]), loss[0] = mean of -(1 - smoothing) log sigmoid(z) -
  *                        smoothing log sigmoid(-z), z = the difference of a pair's rewards.  ws: bmt_preference_ws_bytes, 8-byte aligned; stats at

@@ -153,7 +153,8 @@ def policy_inputs(B, T, V, dtype, g, kl=True, per_token=False):
 
 
 @pytest.mark.parametrize("reduction", ["token", "sequence", "sum"])
-@pytest.mark.parametrize("B,T,V,dtype", [(8, 1, 10000, torch.float32), (4, 29, 1000, torch.float32), (40, 29, 1501, torch.bfloat16), (3, 300, 777, torch.float16),
+@pytest.mark.parametrize("B,T,V,dtype", [(8, 1, 10000, torch.float32), (4, 29, 1000, torch.float32), (150, 130, 17, torch.float32), (3000, 1, 5, torch.bfloat16), (2, 900, 260, torch.float16),
+                                         (1, 20, 32001, torch.bfloat16), (1, 600, 16385, torch.float32), (40, 29, 1501, torch.bfloat16), (3, 300, 777, torch.float16),
                                          (2, 2, 131075, torch.bfloat16), (1, 2, 300001, torch.float32), (700, 1, 4101, torch.float32)])
 def test_policy_loss_and_its_gradient(ops, reduction, B, T, V, dtype):
     g = gen(B * T + V)
@@ -273,6 +274,30 @@ def test_vocabularies_with_forbidden_tokens(ops):
         y[0, 2, 9] = float("inf")
         lp = ops.token_logp(y, ids)          # a row without any probability, a NaN, an infinity: NaN, and only there
         assert bool(torch.isnan(lp[0, :3]).all()) and bool(torch.isfinite(lp[0, 3]))
+
+
+def test_policies_that_lie_far_apart(ops):
+    """ratios from 0 to beyond fp32's exponential: the clipped side where the advantage asks for it, the ratio itself elsewhere"""
+    V, B = 40, 6
+    x = torch.zeros(B, 1, V, device="cuda")
+    x[5, 0, 3] = -float("inf")                      # the sampled token has no probability any more
+    x.requires_grad_(True)
+    ids = torch.full((B, 1), 3, device="cuda")
+    lp = -math.log(V)
+    old = torch.tensor([lp - 3.0, lp + 3.0, lp - 0.4999, lp + 0.5001, lp - 60.0, lp], device="cuda")[:, None]
+    for sign in (1.0, -1.0):
+        adv = torch.full((B,), sign, device="cuda")
+        loss, stats = ops.policy_loss(x, ids, old, adv, reduction="sum")
+        (dx,) = torch.autograd.grad(loss, x)
+        rho = torch.tensor([math.exp(lp - o) for o in old[:5, 0].double().tolist()] + [0.0], dtype=torch.float64, device="cuda")
+        u, c = rho * sign, rho.clamp(0.8, 1.2) * sign
+        want = -torch.minimum(u, c).sum()
+        # lp to (64 + V / 64) u, old to u |old|: the ratios to their sum relatively
+        tol = (66 + abs(lp) + 60) * U
+        within(loss, want, tol * float(rho.sum() if sign < 0 else 8.0), "loss")
+        w = -torch.where(u <= c, u, torch.zeros_like(u))
+        within(dx[:5, 0, 3], w[:5] * (1 - 1 / V), 2 * tol * w[:5].abs(), "dlogits at the tokens")
+        assert float(dx[5].abs().max()) == 0.0
 
 
 def test_on_policy_samples(ops):
