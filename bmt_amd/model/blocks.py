@@ -78,27 +78,16 @@ class VocabularyEmbedder(nn.Module):
                 self.embedder[0].weight.requires_grad = emb_weights_req_grad
 
 
-_ZERO_PE = {}
-
-
-def _zero_pe(S, D, device):
-    key = (S, D, str(device))
-    if key not in _ZERO_PE:
-        _ZERO_PE[key] = torch.zeros(S, D, device=device, dtype=torch.float32)
-    return _ZERO_PE[key]
-
-
 def _embed_table(emb, ids):
-    S, D = ids.shape[1], emb.weight.shape[1]
-    return ops.EmbedFn.apply(ids, emb.weight, _zero_pe(S, D, emb.weight.device), 1.0, 0.0, 0)
+    return ops.embedding(ids.long(), emb.weight)
 
 
 def _embed(vocab_embedder, ids, pe, p, site):
     W = vocab_embedder.embedder.weight
-    S, D = ids.shape[1], W.shape[1]
-    if pe is None:
-        pe = _zero_pe(S, D, W.device)
-    return ops.EmbedFn.apply(ids, W, pe, float(np.sqrt(vocab_embedder.emb_dim)), p, site)
+    scale = float(np.sqrt(vocab_embedder.emb_dim))
+    if pe is None:      # (the plain lookup: a gradient by sorted tokens, the same bits on every run)
+        return ops.embedding(ids.long(), W, scale)
+    return ops.EmbedFn.apply(ids, W, pe, scale, p, site)
 
 
 class FeatureEmbedder(nn.Module):

@@ -21,7 +21,7 @@ import torch
 
 from .loss.label_smoothing import LabelSmoothing
 from .model.masking import mask as make_mask
-from .optim import FusedAdam, clip_grad_norm_
+from .optim import FusedAdam, GradClipper, clip_grad_norm_
 from .parallel import GradientReducer, global_sum
 
 
@@ -102,6 +102,7 @@ class CaptioningTrainStep:
         if hasattr(self.optimizer, "grad_scale"):
             self.optimizer.grad_scale = self.grad_scale
         self._fused_scale = hasattr(self.optimizer, "grad_scale")
+        self._clipper = None            # GradClipper of the arena (cfg.grad_clip with static gradient buffers)
         self._graphs = None
         self._reduce_events = None      # bench: [(start, end)] HIP events around the exposed part of the gradient reduction
         self._flush_points = 0
@@ -179,6 +180,18 @@ class CaptioningTrainStep:
         return _ops.loss_finish(kl, n_global, self.grad_scale), n_global
 
     def _optimize(self):
+        if self.cfg.grad_clip is not None and self._fused_scale and self.reducer is not None:
+            # static gradient buffers: normaliser and clipping in two launches over the arena (what the two passes below leave in p.grad,
+            # from one factor instead of two), the same sums on every run, and nothing in it that a hipGraph cannot replay
+            if self._clipper is None or self._clipper.max_norm != float(self.cfg.grad_clip):
+                self._clipper = GradClipper([self.reducer._arena], self.cfg.grad_clip)
+            self._clipper(scale=self.grad_scale)
+            self.optimizer.grad_scale = None
+            try:
+                self.optimizer.step()
+            finally:
+                self.optimizer.grad_scale = self.grad_scale
+            return
         if not self._fused_scale or self.cfg.grad_clip is not None:
             # generic optimizer, or clipping (which must see the normalised gradients): scale in place first
             for p in self.params:

@@ -704,3 +704,57 @@ def test_caption_model_tuned_on_samples(ops):
     assert abs(after - min(norm, 0.1 * norm / (norm + 1e-6))) <= 8 * U * norm + 1e-9
     opt.step()
     assert any(not torch.equal(a, b) for a, b in zip(before, params)) and all(bool(torch.isfinite(p).all()) for p in params)
+
+
+def caption_step(grad_clip, V=60, B=4, T=9):
+    from bmt_amd import synthetic as syn
+    from bmt_amd.model.captioning_module import BiModalTransformer
+    from bmt_amd.train import CaptioningTrainStep
+    cfg = syn.cfg_config0(dout_p=0.0)
+    cfg.device, cfg.grad_clip, cfg.lr = "cuda:0", grad_clip, 1e-4
+    torch.manual_seed(0)
+    model = BiModalTransformer(cfg, syn.FakeTrainDataset(V, syn.make_glove(V, cfg.d_model_caps))).to("cuda:0")
+    batch = syn.make_cap_batch(cfg, B, 12, 40, T, V, seed=5)
+    fs = {k: v.cuda() for k, v in batch["feature_stacks"].items()}
+    return CaptioningTrainStep(model, cfg, syn.PAD_IDX, static_grads=True), fs, batch["captions"].cuda()
+
+
+@pytest.mark.parametrize("grad_clip", [0.05, 1e6])
+def test_train_step_clips_its_arena(grad_clip):
+    """cfg.grad_clip with static gradient buffers: p.grad holds what normalising and torch's clip_grad_norm_ give, eagerly and in replayed graphs"""
+    step, fs, caps = caption_step(grad_clip)
+    kl, n = step._forward_backward(fs, caps)
+    step._reduce(kl, n)
+    raw = [p.grad.detach().double().clone() for p in step.params]
+    scale = float(step.grad_scale)
+    before = [p.detach().clone() for p in step.params]
+    step._optimize()
+    norm = math.sqrt(sum(float((r * scale).square().sum()) for r in raw))
+    coef = min(1.0, grad_clip / (norm + 1e-6)) * scale
+    for p, r in zip(step.params, raw):
+        within(p.grad, r * coef, 8 * U * (r * coef).abs(), "clipped")          # the factor's roundings and the product's
+    assert step.optimizer.grad_scale is step.grad_scale and any(not torch.equal(a, b) for a, b in zip(before, step.params))
+    step.capture(fs, caps)
+    for _ in range(3):
+        step.replay(fs, caps)
+        torch.cuda.synchronize()
+        total = math.sqrt(sum(float(p.grad.double().square().sum()) for p in step.params))
+        assert 0 < total <= grad_clip * (1 + 1e-5)
+        assert abs(float(step._clipper.coef)) > 0 and all(bool(torch.isfinite(p).all()) for p in step.params)
+        assert grad_clip > 1 or abs(total - grad_clip) <= 1e-4 * grad_clip
+        float(sum(p.sum() for p in step.params))          # (the program's own work between the replays)
+    step.uncapture()
+
+
+def test_vocabulary_embedder_without_positions_uses_the_sorted_gradient(ops):
+    from bmt_amd.model.blocks import VocabularyEmbedder
+    torch.manual_seed(0)
+    emb = VocabularyEmbedder(300, 40).cuda()
+    ids = torch.randint(0, 60, (5, 33), device="cuda", generator=gen(2))
+    up = torch.randn(5, 33, 40, device="cuda", generator=gen(3))
+    W = emb.embedder.weight
+    out = emb(ids)
+    assert torch.equal(out, W.detach()[ids] * torch.tensor(math.sqrt(40), dtype=torch.float32))
+    (dW,) = torch.autograd.grad(out, W, up)
+    _, d64, absum, most = embedding64(ids, W.detach(), math.sqrt(40), up, None)
+    within(dW, d64, (36 + most / 4) * U * absum, "dW")
