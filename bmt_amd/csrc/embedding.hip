@@ -334,14 +334,15 @@ __device__ __forceinline__ void add_rows(const char* dout, int64_t ld, const int
     }
 }
 
-// dW[v] = scale acc, or (into != NULL: a static fp32 gradient buffer) into[v] += scale acc
+// dW[v] = scale acc, or (into != NULL: a static fp32 gradient buffer) into[v] += scale acc -- one addition per row and call, in the memory's own
+// add: another use of the table may be adding its gradient from another stream
 template <int DT, int G>
 __device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, int v, int c, float scale, const float (&acc)[G]) {
     float x[G];
     if (into) {
         float* p = into + (int64_t)v * ldw + c;
 #pragma unroll
-        for (int j = 0; j < G; ++j) p[j] += scale * acc[j];
+        for (int j = 0; j < G; ++j) unsafeAtomicAdd(p + j, scale * acc[j]);
         return;
     }
 #pragma unroll
@@ -528,7 +529,7 @@ extern "C" int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, voi
 }
 
 extern "C" int64_t bmt_embedding_bwd_ws_bytes(int64_t N, int D, int V) {
-    if (N < 0 || N > 0x7fffffff - 64 || D <= 0 || V <= 0) return 0;
+    if (N < 0 || N > 0x7fffffff - 64 || D <= 0 || V <= 0 || V > (1 << 30)) return 0;
     const int64_t chunks = (N + EMB_LONG - 1) / EMB_LONG;
     const Owners ow = owners_for(V);
     const int64_t G = (int64_t)1 << ow.lg;
@@ -538,7 +539,7 @@ extern "C" int64_t bmt_embedding_bwd_ws_bytes(int64_t N, int D, int V) {
 
 extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t ld, int64_t N, int D, int V, int dtype, float scale, int64_t pad_idx, void* dW, float* into,
                                  int64_t ldw, void* ws, int64_t ws_bytes, void* stream) {
-    BMT_CHECK_ARG(known_dtype(dtype) && N >= 0 && N <= 0x7fffffff - 64 && D > 0 && V > 0 && ldw >= D && ld >= 0, "bmt_embedding_bwd: bad args (dtype %d, D %d, V %d)", dtype, D, V);
+    BMT_CHECK_ARG(known_dtype(dtype) && N >= 0 && N <= 0x7fffffff - 64 && D > 0 && V > 0 && V <= (1 << 30) && ldw >= D && ld >= 0, "bmt_embedding_bwd: bad args (dtype %d, D %d, V %d)", dtype, D, V);
     BMT_CHECK_ARG((dW != nullptr) != (into != nullptr), "bmt_embedding_bwd: give either dW or the buffer to add to");
     BMT_CHECK_ARG(!into || dtype == BMT_DT_F32, "bmt_embedding_bwd: only fp32 gradients are added to a buffer");
     BMT_CHECK_ARG(ws && ws_bytes >= bmt_embedding_bwd_ws_bytes(N, D, V) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0,

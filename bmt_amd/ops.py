@@ -3678,6 +3678,11 @@ def _logit_grad_buffer(logits):
     return buf.as_strided(logits.shape, (sb if B > 1 else T * V, st if T > 1 else V, 1), phase)
 
 
+def _recorded(t) -> bool:
+    """whether autograd will ask for t's gradient (inside a Function's forward, needs_input_grad says so under no_grad, too)"""
+    return torch.is_grad_enabled() and t.requires_grad
+
+
 def _last_dim_dense(logits):
     return logits if logits.stride(2) == 1 or logits.shape[2] == 1 else logits.contiguous()
 
@@ -3698,21 +3703,22 @@ class TokenLogpFn(torch.autograd.Function):
     """log_softmax(logits)[ids], per row; the backward recomputes the softmax from the row's maximum and sum"""
 
     @staticmethod
-    def forward(ctx, logits, ids, mask, pad_idx):
+    def forward(ctx, logits, ids, mask, pad_idx, recorded):
         x = _last_dim_dense(logits)
         B, T, _ = x.shape
         logp = torch.empty(B, T, device=x.device, dtype=torch.float32)
-        stats = torch.empty(B, T, 2, device=x.device, dtype=torch.float32) if ctx.needs_input_grad[0] else None
+        stats = torch.empty(B, T, 2, device=x.device, dtype=torch.float32) if recorded else None
         _run_on(x.device, "bmt_logp_rows", lib.bmt_logp_rows, *_row_args(x, ids, mask, pad_idx), logp.data_ptr(), None if stats is None else stats.data_ptr())
-        ctx.save_for_backward(x, ids, mask, stats)
-        ctx.pad_idx = pad_idx
+        if recorded:
+            ctx.save_for_backward(x, ids, mask, stats)
+            ctx.pad_idx = pad_idx
         return logp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d):
         x, ids, mask, stats = ctx.saved_tensors
-        return _logit_grad(x, ids, mask, ctx.pad_idx, stats.data_ptr(), d.data_ptr(), d.stride(0), d.stride(1), None), None, None, None
+        return _logit_grad(x, ids, mask, ctx.pad_idx, stats.data_ptr(), d.data_ptr(), d.stride(0), d.stride(1), None), None, None, None, None
 
 
 def token_logp(logits, ids, mask=None, pad_idx: Optional[int] = None):
@@ -3721,7 +3727,7 @@ def token_logp(logits, ids, mask=None, pad_idx: Optional[int] = None):
     no gradient.  What a policy or preference loss takes as old and reference values."""
     _check_rows("token_logp", logits, ids, mask)
     _tuning_device("token_logp", logits, ids, mask)
-    return TokenLogpFn.apply(logits, ids, mask, pad_idx)
+    return TokenLogpFn.apply(logits, ids, mask, pad_idx, _recorded(logits))
 
 
 class PolicyStats:
@@ -3753,7 +3759,7 @@ class PolicyLossFn(torch.autograd.Function):
     a kernel that ends at once if the upstream gradient IS 1 and computes the gradient again, from the logits, if not"""
 
     @staticmethod
-    def forward(ctx, logits, ids, old, adv, ref, mask, pad_idx, lo, hi, beta, reduction):
+    def forward(ctx, logits, ids, old, adv, ref, mask, pad_idx, lo, hi, beta, reduction, recorded):
         x = _last_dim_dense(logits)
         B, T, V = x.shape
         dev = x.device
@@ -3761,7 +3767,7 @@ class PolicyLossFn(torch.autograd.Function):
         info = torch.empty(2 + B * T, device=dev, dtype=torch.float32)
         n = lib.bmt_policy_ws_bytes(B, T)
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
-        d = _logit_grad_buffer(x) if ctx.needs_input_grad[0] else None
+        d = _logit_grad_buffer(x) if recorded else None
         db, dt = (0, 0) if d is None else (d.stride(0), d.stride(1))
         old, ob, ot = _per_row("policy_loss", "old_logp", old, B, T)
         ref, rb, rt = _per_row("policy_loss", "ref_logp", ref, B, T)
@@ -3780,12 +3786,12 @@ class PolicyLossFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _info):
         if g is None:
-            return (None,) * 11
+            return (None,) * 12
         x, ids, mask, ws = ctx.saved_tensors
         rows = x.shape[0] * x.shape[1]
         out, ctx.dlogits = ctx.dlogits, None      # (a second backward pass through a kept graph computes its own)
         d = _logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr() + 2048 + 16 * rows, ws.data_ptr() + 2048 + 24 * rows, x.shape[1], 1, g, out)
-        return (d,) + (None,) * 10
+        return (d,) + (None,) * 11
 
 
 def policy_loss(logits, ids, old_logp, advantages, ref_logp=None, mask=None, pad_idx: Optional[int] = None, clip_low: float = 0.2,
@@ -3806,15 +3812,17 @@ def policy_loss(logits, ids, old_logp, advantages, ref_logp=None, mask=None, pad
         raise ValueError(f"policy_loss: clip range ({clip_low}, {clip_high})")
     if advantages is None:
         raise ValueError("policy_loss: advantages are needed")
+    if kl_coef != 0 and ref_logp is None:
+        raise ValueError(f"policy_loss: a KL term of {kl_coef} needs ref_logp")
     loss, info = PolicyLossFn.apply(logits, ids, old_logp, advantages, ref_logp, mask, pad_idx, float(clip_low), float(clip_high), float(kl_coef),
-                                    _REDUCTIONS[reduction])
+                                    _REDUCTIONS[reduction], _recorded(logits))
     return loss, PolicyStats(info, ids.shape)
 
 
 class PreferenceLossFn(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, logits, ids, ref, mask, pad_idx, beta, smoothing, mean):
+    def forward(ctx, logits, ids, ref, mask, pad_idx, beta, smoothing, mean, recorded):
         x = _last_dim_dense(logits)
         B, T, V = x.shape
         dev = x.device
@@ -3824,7 +3832,7 @@ class PreferenceLossFn(torch.autograd.Function):
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
         _run_on(dev, "bmt_preference_loss", lib.bmt_preference_loss, *_row_args(x, ids, mask, pad_idx), ref.data_ptr(), ref.stride(0), beta, smoothing,
                 int(mean), loss.data_ptr(), rewards.data_ptr(), ws.data_ptr(), n)
-        if ctx.needs_input_grad[0]:
+        if recorded:
             ctx.save_for_backward(x, ids, mask, ws)
             ctx.pad_idx = pad_idx
         ctx.mark_non_differentiable(rewards)
@@ -3835,10 +3843,10 @@ class PreferenceLossFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _rewards):
         if g is None:
-            return (None,) * 8
+            return (None,) * 9
         x, ids, mask, ws = ctx.saved_tensors
         rows = x.shape[0] * x.shape[1]
-        return (_logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr(), ws.data_ptr() + 8 * rows, 1, 0, g),) + (None,) * 7
+        return (_logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr(), ws.data_ptr() + 8 * rows, 1, 0, g),) + (None,) * 8
 
 
 def preference_loss(logits, ids, ref_logp, mask=None, pad_idx: Optional[int] = None, beta: float = 0.1, label_smoothing: float = 0.0,
@@ -3856,7 +3864,7 @@ def preference_loss(logits, ids, ref_logp, mask=None, pad_idx: Optional[int] = N
         raise ValueError(f"preference_loss: ref_logp of shape {tuple(ref_logp.shape)} and type {ref_logp.dtype} (float32 ({B},))")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"preference_loss: label_smoothing {label_smoothing}")
-    return PreferenceLossFn.apply(logits, ids, ref_logp, mask, pad_idx, float(beta), float(label_smoothing), bool(mean_logp))
+    return PreferenceLossFn.apply(logits, ids, ref_logp, mask, pad_idx, float(beta), float(label_smoothing), bool(mean_logp), _recorded(logits))
 
 
 def _embedding_forward(idc, W, scale):
@@ -3907,7 +3915,7 @@ def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
     gradient of ``weight`` is added in fp32 over a token's positions in ascending order and rounded once -- the same bits on every run, whichever
     tokens repeat --; ``pad_idx`` gets none.  A parameter with a static gradient buffer (GradientReducer) has it added there directly."""
     _tuning_device("embedding", ids, weight)
-    if weight.dim() != 2 or weight.dtype not in _DTYPES or weight.shape[0] == 0 or weight.shape[1] == 0:
+    if weight.dim() != 2 or weight.dtype not in _DTYPES or not 0 < weight.shape[0] <= 1 << 30 or weight.shape[1] == 0:
         raise ValueError(f"embedding: a weight of shape {tuple(weight.shape)} and type {weight.dtype} (2-D float32, bfloat16 or float16)")
     if ids.dtype != torch.int64:
         raise ValueError(f"embedding: ids of type {ids.dtype} (int64)")
@@ -3916,6 +3924,6 @@ def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
     if weight.stride(0) < weight.shape[1] or (weight.shape[1] > 1 and weight.stride(1) != 1):
         weight = weight.contiguous()
     idc = ids.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if _recorded(weight):
         return EmbeddingFn.apply(idc, weight, float(scale), pad_idx)
     return _embedding_forward(idc, weight, float(scale))

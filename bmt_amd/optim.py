@@ -138,6 +138,7 @@ def clip_grad_norm_(parameters: Iterable[torch.nn.Parameter], max_norm: float) -
     return sq.sqrt().squeeze(0)
 
 
+_captured_tables = []   # tile tables that a captured hipGraph may still read: never freed (24 bytes per 32 KB of gradients)
 CLIP_TILE = 32768       # bytes of gradient per tile of GradClipper's table: 128 per thread of a workgroup
 
 
@@ -232,6 +233,8 @@ class GradClipper:
             raise RuntimeError("GradClipper: a tensor's memory has moved since the plan was made: make a new one")
         if scale is not None and (scale.numel() != 1 or scale.dtype != torch.float32 or scale.device != self.device):
             raise ValueError(f"GradClipper: scale is one float32 value on {self.device}")
+        if torch.cuda.is_current_stream_capturing() and not any(t is self._tiles for t in _captured_tables):
+            _captured_tables.append(self._tiles)
         result = torch.empty(2, device=self.device, dtype=torch.float32)
         n = lib.bmt_clip_ws_bytes()
         ws = torch.empty(n, device=self.device, dtype=torch.uint8)      # (of this call: two captured graphs, or two streams, share nothing)

@@ -251,6 +251,18 @@ def test_rows_that_do_not_count_leak_nothing(ops):
         assert bool(torch.isnan(ops.token_logp(x.detach(), ids)[0, 0])) and bool(torch.isnan(ops.policy_loss(x, ids, old, adv, ref, None, PAD)[0]))
 
 
+def test_nothing_is_held_where_no_graph_is_recorded(ops):
+    x = torch.randn(4, 64, 4096, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 4096, (4, 64), device="cuda")
+    row, seq = torch.zeros(4, 64, device="cuda"), torch.zeros(4, device="cuda")
+    for call in (lambda: ops.policy_loss(x, ids, row, seq), lambda: ops.preference_loss(x, ids, seq), lambda: ops.token_logp(x, ids)):
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        with torch.no_grad():
+            call()
+        assert torch.cuda.max_memory_allocated() - held < x.numel() * 4 // 8
+
+
 def test_vocabularies_with_forbidden_tokens(ops):
     """-inf and the type's lowest value among the logits: probability 0 and gradient 0 there, and a row of nothing but the lowest value is uniform"""
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
@@ -570,7 +582,7 @@ def test_losses_refuse_device_tensors_of_the_wrong_kind(ops):
     x, ids = torch.zeros(2, 3, 5, device="cuda"), torch.zeros(2, 3, device="cuda", dtype=torch.int64)
     row = torch.zeros(2, 3, device="cuda")
     for kw in (dict(advantages=None), dict(advantages=torch.zeros(3, device="cuda")), dict(advantages=row.double()), dict(old_logp=row[:, :1]), dict(ref_logp=row[0]),
-               dict(reduction="mean"), dict(clip_low=-0.1), dict(clip_high=float("nan"))):
+               dict(reduction="mean"), dict(kl_coef=0.1), dict(clip_low=-0.1), dict(clip_high=float("nan"))):
         with pytest.raises(ValueError):
             ops.policy_loss(x, ids, **{"old_logp": row, "advantages": row, **kw})
     with pytest.raises(RuntimeError, match="no CPU fallback"):
@@ -624,6 +636,19 @@ def test_a_step_on_a_side_stream_and_in_a_graph(ops):
             side.synchronize()
             assert all(torch.equal(x, y) for x, y in zip(got, w))
     static = [t.clone() for t in batches[0]]
+    side = torch.cuda.Stream()
+    alone = torch.cuda.CUDAGraph()
+    lonely = [torch.full((5000,), 3.0, device="cuda")]
+    plans = [GradClipper(lonely, 1.0)]
+    with torch.cuda.graph(alone):          # a graph that outlives its plan
+        norm = plans.pop()()
+    junk = [torch.full((4096,), float("nan"), device="cuda") for _ in range(64)]
+    for _ in range(2):
+        lonely[0].fill_(3.0)
+        alone.replay()
+        torch.cuda.synchronize()
+        assert abs(float(norm) - 3.0 * math.sqrt(5000)) < 1e-3 and abs(float(lonely[0].norm()) - 1.0) < 1e-5
+    del junk
     clippers = [GradClipper([torch.zeros_like(W).detach(), torch.zeros_like(head).detach()], 0.01) for _ in range(2)]
     graphs, outs = [], []
     side = torch.cuda.Stream()
