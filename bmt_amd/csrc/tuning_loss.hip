@@ -70,21 +70,12 @@ struct Elem<BMT_DT_F16> {
     static __device__ __forceinline__ float get1(const char* p) { return h_bits2f(*reinterpret_cast<const uint16_t*>(p)); }
 };
 
-// e^t, t <= 0 (NaN stays NaN): the instruction's 2^y of y = t log2 e, log2 e as the sum of two floats.  The instruction is right to 2.6e-8 (rms); y's
-// rounding adds 3e-8 |t|
+// e^t, t <= 0 (NaN stays NaN): the instruction's 2^y of y = t log2 e, log2 e as the sum of two floats.  The instruction is right to 2.6e-8 (rms; its
+// mean over evenly spread y is EXP_BIAS low), y's rounding adds 3e-8 |t|
+constexpr double EXP_BIAS = 3.3e-9;
 __device__ __forceinline__ float exp_neg(float t) {
     return __builtin_amdgcn_exp2f(__fmaf_rn(t, 1.44269502162933349609375f, t * 1.92596299112661746e-8f));
 }
-// the same with what y's rounding lost put back to first order: 2^(y + l) = 2^y (1 + l ln 2), for factors whose error does not average out: 16-bit
-// logits leave few different maxima, every row of a sequence repeats the same few factors, and the errors of hundreds of rows add up (rewards of
-// 1024-token sequences were off by 1.4e-6 of their size; 3e-7 now).  (t = -inf: l is NaN, the median takes it to -1, and 2^y is 0)
-__device__ __forceinline__ float exp_neg_exact(float t) {
-    const float y = t * 1.44269502162933349609375f;
-    const float l = __fmaf_rn(t, 1.92596299112661746e-8f, __fmaf_rn(t, 1.44269502162933349609375f, -y));
-    const float e = __builtin_amdgcn_exp2f(y);
-    return __fmaf_rn(e, __builtin_amdgcn_fmed3f(l, -1.f, 1.f) * 0.693147180559945309f, e);
-}
-
 // the (B, T) rows of a call: logits with two row strides, ids and an optional mask with theirs (all strides in elements)
 struct Rows {
     const char* x;
@@ -360,7 +351,13 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
     }
     float xt = __builtin_nanf("");      // an id outside the vocabulary has no log-probability
     if (threadIdx.x == 0 && id >= 0 && id < q.V) xt = E::get1(xr + id * E::B);
-    float m = -__builtin_huge_valf(), s = 0.f;
+    // A thread's exponentials are taken against its running maximum plus a fraction of its own, ms.  Logits of 16 bits leave few different distances
+    // from a maximum; every row of a sequence would repeat the same few rounding errors, and a sequence's log-probability add hundreds of them up
+    // (rewards of 1024 tokens were off by up to 2e-6 of their size).  Spread like this they average out, and EXP_BIAS is what is left of them; the
+    // maximum itself, nearly the whole sum in a peaked row, is put back as the 1 that it is
+    const float spread = (float)((((uint32_t)r * 0x9E3779B1u) ^ (threadIdx.x * 0x85EBCA6Bu)) >> 20) * 0x1p-12f;
+    float m = -__builtin_huge_valf(), ms = 0.f;
+    double s = 0.0;
     for (int k0 = threadIdx.x; k0 < n; k0 += NT * U) {
         u32x4 v[U];
         const uint32_t l = E::lowest();
@@ -376,20 +373,25 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
 #pragma unroll
             for (int j = 0; j < E::G; ++j) bm = fmaxf(bm, x[i][j]);
         }
-        const float mn = fmaxf(m, bm), ms = mn == -__builtin_huge_valf() ? 0.f : mn;      // (nothing but -inf so far: the sum stays 0)
-        s *= exp_neg(m - ms);
+        m = fmaxf(m, bm);
+        const float ns = m == -__builtin_huge_valf() ? 0.f : m + spread;      // (nothing but -inf so far: the sum stays 0)
+        s = s == 0.0 ? 0.0 : s * (double)exp_neg(ms - ns);
+        ms = ns;
         float a = 0.f;
 #pragma unroll
         for (int i = 0; i < U; ++i)
 #pragma unroll
             for (int j = 0; j < E::G; ++j) a += exp_neg(x[i][j] - ms);
-        s += a;
-        m = mn;
+        s += (double)a;
     }
     double norm = 1.0;
     if constexpr (POLICY) norm = row_norm(p, group_count<NT>(cnt.share(q, p), redi));
     const float M = group_max<NT>(m, redf);
-    const double S = group_sum<NT>(m == -__builtin_huge_valf() ? (double)s : (double)s * (double)exp_neg_exact(m - M), redd);
+    if (s != 0.0) {      // (NaN, too)
+        const double f = exp((double)ms - (double)M);
+        s = (s - (m == M ? (double)exp_neg(m - ms) : 0.0)) * f * (1.0 + EXP_BIAS) + (m == M ? 1.0 : 0.0);
+    }
+    const double S = group_sum<NT>(s, redd);
     if (threadIdx.x == 0) {
         const double lp = ((double)xt - (double)M) - log(S);
         if (logp) logp[r] = (float)lp;
