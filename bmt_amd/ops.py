@@ -3606,14 +3606,15 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i:
 
 def _tuning_device(who: str, *tensors):
     """refuses tensors (None: absent) that are not all on one GPU"""
-    dev = tensors[0].device
+    first = tensors[0].get_device()
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()          # (-1: not on a GPU)
+        if d < 0:
             raise RuntimeError(f"{who}: bmt_amd ops need CUDA/HIP tensors: there is no CPU fallback (use the oracle for CPU checks)")
-        if t.device != dev:
-            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
+        if d != first:
+            raise ValueError(f"{who}: tensors on {tensors[0].device} and {t.device}")
 
 
 def _run_on(dev: torch.device, what: str, fn, *args):
@@ -3629,7 +3630,8 @@ def _run_on(dev: torch.device, what: str, fn, *args):
 
 
 def _check_rows(who: str, logits, ids, mask):
-    if logits.dim() != 3 or ids.shape != logits.shape[:2]:
+    shape = logits.shape
+    if len(shape) != 3 or ids.shape != shape[:2]:
         raise ValueError(f"{who}: logits (B, T, V) and ids (B, T), not {tuple(logits.shape)} and {tuple(ids.shape)}")
     if logits.dtype not in _DTYPES:
         raise ValueError(f"{who}: logits of type {logits.dtype} (float32, bfloat16 or float16)")
@@ -3637,8 +3639,8 @@ def _check_rows(who: str, logits, ids, mask):
         raise ValueError(f"{who}: ids of type {ids.dtype} (int64)")
     if mask is not None and (mask.shape != ids.shape or mask.dtype not in (torch.bool, torch.uint8)):
         raise ValueError(f"{who}: mask of shape {tuple(mask.shape)} and type {mask.dtype} (a bool or uint8 one of {tuple(ids.shape)})")
-    if logits.shape[2] == 0 or logits.shape[2] > 1 << 30:
-        raise ValueError(f"{who}: a vocabulary of {logits.shape[2]} tokens")
+    if shape[2] == 0 or shape[2] > 1 << 30:
+        raise ValueError(f"{who}: a vocabulary of {shape[2]} tokens")
 
 
 def _per_row(who: str, name: str, t, B: int, T: int, per_sequence: bool = False):
@@ -3655,9 +3657,8 @@ def _per_row(who: str, name: str, t, B: int, T: int, per_sequence: bool = False)
 
 
 def _row_args(logits, ids, mask, pad_idx):
-    B, T, V = logits.shape
     mb, mt = (0, 0) if mask is None else mask.stride()
-    return (logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), logits.stride(1), B, T, V, ids.data_ptr(), ids.stride(0), ids.stride(1),
+    return (logits.data_ptr(), _DTYPES[logits.dtype], *logits.stride()[:2], *logits.shape, ids.data_ptr(), *ids.stride(),
             None if mask is None else mask.data_ptr(), mb, mt, _NO_PAD if pad_idx is None else int(pad_idx))
 
 
@@ -3736,7 +3737,7 @@ class PolicyStats:
     __slots__ = ("_buf", "_shape")
 
     def __init__(self, buf, shape):
-        self._buf, self._shape = buf, shape          # KL, clip fraction, log-probabilities
+        self._buf, self._shape = buf, shape          # KL, clip fraction, log-probabilities; behind them the loss's workspace
 
     @property
     def kl(self):
@@ -3748,7 +3749,7 @@ class PolicyStats:
 
     @property
     def logp(self):
-        return self._buf[2:].view(self._shape)
+        return self._buf[4:4 + self._shape[0] * self._shape[1]].view(self._shape)
 
 
 _REDUCTIONS = {"sum": 0, "token": 1, "sequence": 2}
@@ -3764,20 +3765,21 @@ class PolicyLossFn(torch.autograd.Function):
         B, T, V = x.shape
         dev = x.device
         loss = torch.empty((), device=dev, dtype=torch.float32)
-        info = torch.empty(2 + B * T, device=dev, dtype=torch.float32)
         n = lib.bmt_policy_ws_bytes(B, T)
-        ws = torch.empty(n, device=dev, dtype=torch.uint8)
+        at = (4 + B * T + 3) // 4 * 4          # KL, clip fraction, log-probabilities | 16-byte aligned workspace
+        info = torch.empty(at + (n + 3) // 4, device=dev, dtype=torch.float32)
+        ws = info.data_ptr() + 4 * at
         d = _logit_grad_buffer(x) if recorded else None
         db, dt = (0, 0) if d is None else (d.stride(0), d.stride(1))
         old, ob, ot = _per_row("policy_loss", "old_logp", old, B, T)
         ref, rb, rt = _per_row("policy_loss", "ref_logp", ref, B, T)
-        adv, ab, at = _per_row("policy_loss", "advantages", adv, B, T, per_sequence=True)
+        adv, ab, av = _per_row("policy_loss", "advantages", adv, B, T, per_sequence=True)
         _run_on(dev, "bmt_policy_loss", lib.bmt_policy_loss, *_row_args(x, ids, mask, pad_idx), None if old is None else old.data_ptr(), ob, ot,
-                None if ref is None else ref.data_ptr(), rb, rt, adv.data_ptr(), ab, at, lo, hi, beta, reduction, loss.data_ptr(), info.data_ptr(),
-                info.data_ptr() + 8, ws.data_ptr(), n, None if d is None else d.data_ptr(), db, dt)
+                None if ref is None else ref.data_ptr(), rb, rt, adv.data_ptr(), ab, av, lo, hi, beta, reduction, loss.data_ptr(), info.data_ptr(),
+                info.data_ptr() + 16, ws, n, None if d is None else d.data_ptr(), db, dt)
         if d is not None:
-            ctx.save_for_backward(x, ids, mask, ws)
-            ctx.pad_idx, ctx.dlogits = pad_idx, d
+            ctx.save_for_backward(x, ids, mask)
+            ctx.pad_idx, ctx.dlogits, ctx.info, ctx.ws = pad_idx, d, info, ws          # (info: an output, held for its workspace)
         ctx.mark_non_differentiable(info)
         ctx.set_materialize_grads(False)
         return loss, info
@@ -3787,10 +3789,10 @@ class PolicyLossFn(torch.autograd.Function):
     def backward(ctx, g, _info):
         if g is None:
             return (None,) * 12
-        x, ids, mask, ws = ctx.saved_tensors
+        x, ids, mask = ctx.saved_tensors
         rows = x.shape[0] * x.shape[1]
         out, ctx.dlogits = ctx.dlogits, None      # (a second backward pass through a kept graph computes its own)
-        d = _logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr() + 2048 + 16 * rows, ws.data_ptr() + 2048 + 24 * rows, x.shape[1], 1, g, out)
+        d = _logit_grad(x, ids, mask, ctx.pad_idx, ctx.ws + 2048 + 16 * rows, ctx.ws + 2048 + 24 * rows, x.shape[1], 1, g, out)
         return (d,) + (None,) * 11
 
 
