@@ -9,6 +9,9 @@
 //   sum    a wave per (token, block of columns) adds a token's rows if they are at most EMB_LONG; the rows of more frequent tokens are added
 //          EMB_LONG sorted positions at a time by workgroups of their own (a few tokens hold half of a text)
 //   join   adds those partial sums per token, in order
+// Measured (bf16, 65536 Zipf-distributed ids, 32000 x 1024 table): lookup 29 us (6.9 TB/s of distinct rows read + rows written); gradient 67 us for
+// 200 MB: order 17 us in three launches, sum 37 us (5.4 TB/s), join 5 us.  An odd width (1021) costs the same within 2 us (93 and 129 us when such
+// rows were read element by element).
 #include "common.h"
 
 namespace {
@@ -38,19 +41,19 @@ struct Vec;
 template <>
 struct Vec<16> { typedef u32x4 T; };
 template <>
-struct Vec<8> { typedef u32x2 T; };
-template <>
 struct Vec<4> { typedef uint32_t T; };
 template <>
 struct Vec<2> { typedef uint16_t T; };
 
 template <int DT>
 constexpr int elem_size() { return DT == BMT_DT_F32 ? 4 : 2; }
-// G elements (16, 8 or one element's bytes) at p <-> floats
+// G elements at p <-> floats: 16 bytes at any address of an element (rows of odd widths start anywhere; the hardware takes such accesses), or one
+// element where a row does not hold 16 bytes
 template <int DT, int G>
 struct Cols {
     typedef typename Vec<elem_size<DT>() * G>::T T;
-    static __device__ __forceinline__ T load(const char* p) { return *reinterpret_cast<const T*>(p); }
+    typedef T Anywhere __attribute__((aligned(elem_size<DT>())));
+    static __device__ __forceinline__ T load(const char* p) { return *reinterpret_cast<const Anywhere*>(p); }
     static __device__ __forceinline__ uint32_t word(const T& v, int i) {
         if constexpr (sizeof(T) <= 4) return (uint32_t)v;
         else return v[i];
@@ -81,24 +84,32 @@ struct Cols {
 #pragma unroll
             for (int j = 0; j < G / 2; ++j) v[j] = pack_2<DT == BMT_DT_F16>(x[2 * j], x[2 * j + 1]);
         }
-        __builtin_nontemporal_store(v, reinterpret_cast<T*>(p));
+        __builtin_nontemporal_store(v, reinterpret_cast<Anywhere*>(p));
     }
 };
+
+// the G columns of a lane, of which the first would be c: a row's last lane steps back to columns that others hold, too (they get the same values)
+template <int G>
+__device__ __forceinline__ int cols_at(int c, int D) { return min(c, D - G); }
 
 // ---------------------------------------------------------------- lookup: a wave per (TPW tokens, block of 64 G columns)
 template <int DT, int G, int TPW>
 __global__ __launch_bounds__(256) void embed_kernel(const int64_t* __restrict__ ids, const char* __restrict__ W, int64_t ldw, char* __restrict__ out, int64_t N, int D,
                                                      int V, float scale, int ncb, int64_t tasks) {
     constexpr int E = elem_size<DT>();
-    const int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (task >= tasks) return;
+    const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);      // (uniform: the ids are scalar loads, and no row's
+    if (task >= tasks) return;                                                                            // load waits behind another's id)
     const int64_t n0 = task / ncb * TPW;
-    const int c = ((int)(task % ncb) * 64 + (threadIdx.x & 63)) * G;
+    int c = ((int)(task % ncb) * 64 + (threadIdx.x & 63)) * G;
     if (c >= D) return;
+    c = cols_at<G>(c, D);
     typename Cols<DT, G>::T v[TPW];
+    int64_t row[TPW];
+#pragma unroll
+    for (int i = 0; i < TPW; ++i) row[i] = n0 + i < N ? (int64_t)clamp_id(ids[n0 + i], V) * ldw : 0;
 #pragma unroll
     for (int i = 0; i < TPW; ++i)
-        if (n0 + i < N) v[i] = Cols<DT, G>::load(W + ((int64_t)clamp_id(ids[n0 + i], V) * ldw + c) * E);
+        if (n0 + i < N) v[i] = Cols<DT, G>::load(W + (row[i] + c) * E);
 #pragma unroll
     for (int i = 0; i < TPW; ++i)
         if (n0 + i < N) {
@@ -112,9 +123,10 @@ __global__ __launch_bounds__(256) void embed_kernel(const int64_t* __restrict__ 
 
 // ---------------------------------------------------------------- order: stable counting sort, an owner's tokens per workgroup
 // Wave w walks the ids [w * chunk, (w + 1) * chunk); K > 0: a lane keeps its K ids in registers between counting and placing (N <= 1024 K),
-// K = 0: they are read twice; K = -1: the owner's ids were split off (sp).  offsets[u] = first sorted position of the token in slot u, offsets[slots] = the positions that count (the padding
-// id does not).  Placing 64 positions: the lanes that hold one token find each other by a ballot per bit of its number -- the cost does not depend
-// on how many different tokens they hold (one round per different token took 245 us for 65536 Zipf-distributed ids, 10 times as long).
+// K = 0: they are read twice; K = -1: the owner's ids were split off (sp).  offsets[u] = first sorted position of the token in slot u,
+// offsets[slots] = the positions that count (the padding id does not).  Placing 64 positions: the lanes that hold one token find each other by a
+// ballot per bit of its number -- the cost does not depend on how many different tokens they hold (a round per different token: 245 us for 65536
+// Zipf-distributed ids, against 57).
 template <int K>
 __global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __restrict__ ids, int64_t N, int V, int64_t pad, Owners ow, int bits, int slots, Split sp,
                                                             int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ slot) {
@@ -318,7 +330,7 @@ __device__ __forceinline__ void add_rows(const char* dout, int64_t ld, const int
                 const int n = __builtin_amdgcn_readlane(pos, min(i + u, have - 1));
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
-                    if (c + j * 64 * G < D && i + u < have) v[u][j] = Cols<DT, G>::load(dout + ((int64_t)n * ld + c + j * 64 * G) * E);
+                    if (c + j * 64 * G < D && i + u < have) v[u][j] = Cols<DT, G>::load(dout + ((int64_t)n * ld + cols_at<G>(c + j * 64 * G, D)) * E);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -337,17 +349,19 @@ __device__ __forceinline__ void add_rows(const char* dout, int64_t ld, const int
 // dW[v] = scale acc, or (into != NULL: a static fp32 gradient buffer) into[v] += scale acc -- one addition per row and call, in the memory's own
 // add: another use of the table may be adding its gradient from another stream
 template <int DT, int G>
-__device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, int v, int c, float scale, const float (&acc)[G]) {
+__device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, int v, int c, int D, float scale, const float (&acc)[G]) {
     float x[G];
+    const int at = cols_at<G>(c, D);
     if (into) {
-        float* p = into + (int64_t)v * ldw + c;
+        float* p = into + (int64_t)v * ldw + at;
 #pragma unroll
-        for (int j = 0; j < G; ++j) unsafeAtomicAdd(p + j, scale * acc[j]);
+        for (int j = 0; j < G; ++j)
+            if (at + j >= c) unsafeAtomicAdd(p + j, scale * acc[j]);      // (each column once)
         return;
     }
 #pragma unroll
     for (int j = 0; j < G; ++j) x[j] = scale * acc[j];
-    Cols<DT, G>::store(dW + ((int64_t)v * ldw + c) * elem_size<DT>(), x);
+    Cols<DT, G>::store(dW + ((int64_t)v * ldw + at) * elem_size<DT>(), x);
 }
 
 // the four waves' sums into wave 0, in order
@@ -395,7 +409,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
                     if (c + j * 64 * G < D) {
-                        float* o = part + (int64_t)(2 * k + h) * ldp + c + j * 64 * G;
+                        float* o = part + (int64_t)(2 * k + h) * ldp + cols_at<G>(c + j * 64 * G, D);
 #pragma unroll
                         for (int g = 0; g < G; ++g) o[g] = acc[j][g];
                     }
@@ -412,7 +426,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
         add_rows<DT, G, NB>(dout, ld, order, a, b, c, D, acc);
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            if (c + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, v, c + j * 64 * G, scale, acc[j]);
+            if (c + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, v, c + j * 64 * G, D, scale, acc[j]);
     }
     if (chunks) return;
     // no partial sums: the four waves share each frequent token that one of them met
@@ -430,7 +444,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
         if (wave == 0)
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-                if (mc + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, m.z, mc + j * 64 * G, scale, acc[j]);
+                if (mc + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, m.z, mc + j * 64 * G, D, scale, acc[j]);
     }
 }
 
@@ -452,26 +466,20 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__
     if (in) {
 #pragma unroll 4
         for (int i = i0; i < i1; ++i) {
-            const float* o = part + (int64_t)(2 * (k + i) + (i == 0 && a > p0 ? 1 : 0)) * ldp + c;
+            const float* o = part + (int64_t)(2 * (k + i) + (i == 0 && a > p0 ? 1 : 0)) * ldp + cols_at<G>(c, D);
 #pragma unroll
             for (int j = 0; j < G; ++j) acc[0][j] += o[j];
         }
     }
     join_waves<G, 1>(acc, red, wave, lane);
-    if (wave == 0 && in) finish_row<DT, G>(dW, into, ldw, ow.token(u), c, scale, acc[0]);
+    if (wave == 0 && in) finish_row<DT, G>(dW, into, ldw, ow.token(u), c, D, scale, acc[0]);
 }
 
 inline int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 inline int64_t emb_ld(int D) { return (D + 7) / 8 * 8; }      // floats per partial sum: 16-byte rows for every G
 
-// elements per lane: 16 or 8 bytes where every row of both sides is aligned to them, else one element
-inline int cols_of(int esize, int D, const void* a, int64_t lda, const void* b, int64_t ldb) {
-    for (int bytes = 16; bytes >= 8; bytes /= 2) {
-        const int64_t g = bytes / esize;
-        if (D % g == 0 && lda % g == 0 && ldb % g == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & (bytes - 1)) == 0) return (int)g;
-    }
-    return 1;
-}
+// elements per lane: 16 bytes, or one where a row is shorter than that
+inline int cols_of(int esize, int D) { return D >= 16 / esize ? 16 / esize : 1; }
 
 // one workgroup per CU: each reads every id once, so more of them only multiply the reads
 inline Owners owners_for(int V) {
@@ -486,21 +494,18 @@ inline int split_rounds(int64_t N) { return N <= 256 * 1024 ? 1 : N <= 1024 * 10
 inline int64_t split_chunks(int64_t N) { return (N + 1024 * split_rounds(N) - 1) / (1024 * split_rounds(N)); }
 inline int groups_for(const Owners& ow, int V) { return V < (1 << ow.lg) ? V : 1 << ow.lg; }
 
-#define BMT_EMB_BY(dtype, g, CALL)                                                           \
-    do {                                                                                     \
-        if (dtype == BMT_DT_F32) {                                                           \
-            if (g == 4) CALL(BMT_DT_F32, 4);                                                 \
-            else if (g == 2) CALL(BMT_DT_F32, 2);                                            \
-            else CALL(BMT_DT_F32, 1);                                                        \
-        } else if (dtype == BMT_DT_BF16) {                                                   \
-            if (g == 8) CALL(BMT_DT_BF16, 8);                                                \
-            else if (g == 4) CALL(BMT_DT_BF16, 4);                                           \
-            else CALL(BMT_DT_BF16, 1);                                                       \
-        } else {                                                                             \
-            if (g == 8) CALL(BMT_DT_F16, 8);                                                 \
-            else if (g == 4) CALL(BMT_DT_F16, 4);                                            \
-            else CALL(BMT_DT_F16, 1);                                                        \
-        }                                                                                    \
+#define BMT_EMB_BY(dtype, g, CALL)                  \
+    do {                                            \
+        if (dtype == BMT_DT_F32) {                  \
+            if (g == 4) CALL(BMT_DT_F32, 4);        \
+            else CALL(BMT_DT_F32, 1);               \
+        } else if (dtype == BMT_DT_BF16) {          \
+            if (g == 8) CALL(BMT_DT_BF16, 8);       \
+            else CALL(BMT_DT_BF16, 1);              \
+        } else {                                    \
+            if (g == 8) CALL(BMT_DT_F16, 8);        \
+            else CALL(BMT_DT_F16, 1);               \
+        }                                           \
     } while (0)
 
 inline bool known_dtype(int d) { return d == BMT_DT_F32 || d == BMT_DT_BF16 || d == BMT_DT_F16; }
@@ -511,7 +516,8 @@ extern "C" int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, voi
     BMT_CHECK_ARG(known_dtype(dtype) && N >= 0 && D > 0 && V > 0 && ldw >= D, "bmt_embedding: bad args (dtype %d, D %d, V %d)", dtype, D, V);
     if (N == 0) return BMT_OK;
     BMT_CHECK_ARG(ids && W && out, "bmt_embedding: null pointer");
-    const int es = dtype == BMT_DT_F32 ? 4 : 2, g = cols_of(es, D, W, ldw, out, D), ncb = bmt_cdiv(D, 64 * g);
+    BMT_CHECK_ARG(((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(out)) & (dtype == BMT_DT_F32 ? 3 : 1)) == 0, "bmt_embedding: not aligned to the elements");
+    const int es = dtype == BMT_DT_F32 ? 4 : 2, g = cols_of(es, D), ncb = bmt_cdiv(D, 64 * g);
     const int tpw = N >= 16384 ? 4 : 1;      // enough waves to fill the chip: four tokens' loads in flight in each
     const int64_t tasks = (N + tpw - 1) / tpw * ncb, grid = (tasks + 3) / 4;
     BMT_CHECK_ARG(grid <= 0x7fffffff, "bmt_embedding: too many tokens");
@@ -545,6 +551,8 @@ extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t l
     BMT_CHECK_ARG(ws && ws_bytes >= bmt_embedding_bwd_ws_bytes(N, D, V) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0,
                   "bmt_embedding_bwd: workspace of %lld bytes is too small or not aligned", (long long)ws_bytes);
     BMT_CHECK_ARG((ids && dout) || N == 0, "bmt_embedding_bwd: null pointer");
+    BMT_CHECK_ARG(((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dW) | reinterpret_cast<uintptr_t>(into)) & (dtype == BMT_DT_F32 ? 3 : 1)) == 0,
+                  "bmt_embedding_bwd: not aligned to the elements");
     if (N == 0 && into) return BMT_OK;
     hipStream_t st = (hipStream_t)stream;
     const Owners ow = owners_for(V);
@@ -554,7 +562,7 @@ extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t l
     int* slot = (int*)((char*)order + round16(N * 4));
     float* part = (float*)((char*)slot + round16(N * 4));
     const int es = dtype == BMT_DT_F32 ? 4 : 2;
-    const int g = cols_of(es, D, dout, ld, into ? (void*)into : dW, ldw), ncb = bmt_cdiv(D, 64 * g), nb2 = ncb >= 2 ? 2 : 1, ncs = bmt_cdiv(ncb, nb2);
+    const int g = cols_of(es, D), ncb = bmt_cdiv(D, 64 * g), nb2 = ncb >= 2 ? 2 : 1, ncs = bmt_cdiv(ncb, nb2);
     const int64_t chunks = N > EMB_FEW ? (N + EMB_LONG - 1) / EMB_LONG : 0;
     const int64_t grid = chunks * ncs + ((int64_t)V * ncs + 3) / 4;
     const int64_t ldp = emb_ld(D);

@@ -197,13 +197,13 @@ struct Row {
     }
 };
 
-// writes granule k of the row to `out` (same phase: 16-byte stores; another one: element by element)
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+// writes granule k of the row to `out`, 16 bytes at whatever address of an element that is (the hardware takes it); the edges element by element
 template <int DT>
-__device__ __forceinline__ void put_granule(const Row<DT>& row, int k, const u32x4& v, char* out, bool same) {
-    if (same && row.inner(k)) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out + ((int64_t)k * Elem<DT>::G - row.phase) * Elem<DT>::B));
+__device__ __forceinline__ void put_granule(const Row<DT>& row, int k, const u32x4& v, char* out) {
+    if (row.inner(k)) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(out + ((int64_t)k * Elem<DT>::G - row.phase) * Elem<DT>::B));
     else row.store_elements(k, v, out);
 }
-__device__ __forceinline__ bool same_phase(const char* a, const char* b) { return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0; }
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     char* dr = dx + (b * db + t * dt) * E::B;
     if (!row_counts(q, b, t, id)) {
         const Row<DT> o(dr, q.V);
-        for (int k = threadIdx.x, n = o.granules(); k < n; k += NT) put_granule<DT>(o, k, u32x4{0, 0, 0, 0}, dr, true);
+        for (int k = threadIdx.x, n = o.granules(); k < n; k += NT) put_granule<DT>(o, k, u32x4{0, 0, 0, 0}, dr);
         if (threadIdx.x == 0) {
             logp[r] = 0.f;
             stats[r] = make_float2(0.f, 0.f);
@@ -488,7 +488,6 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     __syncthreads();
     const float wr = wc[0], c = -wr * wc[1];
     const int kt = (int)((row.phase + id) / E::G), jt = (int)((row.phase + id) % E::G);      // (outside the vocabulary: wr is NaN everywhere)
-    const bool same = same_phase(xr, dr);
     int k0 = threadIdx.x;
     asm volatile("" : "+v"(k0));      // (the places of the stores are worked out anew, not kept from the loads: two registers per granule)
 #pragma unroll
@@ -504,7 +503,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
                 for (int j = 0; j < E::G; ++j)
                     if (j == jt) x[j] += wr;
             }
-            put_granule<DT>(row, k, E::put(x), dr, same);
+            put_granule<DT>(row, k, E::put(x), dr);
         }
     }
 }
@@ -570,7 +569,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
         char* dr = dx + (b * db + t * dt) * E::B;
         if (!row_counts(q, b, t, id)) {
             const Row<DT> o(dr, q.V);
-            for (int k = threadIdx.x, n = o.granules(); k < n; k += NT) put_granule<DT>(o, k, u32x4{0, 0, 0, 0}, dr, true);
+            for (int k = threadIdx.x, n = o.granules(); k < n; k += NT) put_granule<DT>(o, k, u32x4{0, 0, 0, 0}, dr);
             continue;
         }
         const Row<DT> row(xr, q.V);
@@ -578,8 +577,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
         const float2 st = stats[r];
         const float wr = w[b * wb + t * wt] * gs, m = st.x, c = -wr * st.y;
         const int kt = (int)((row.phase + id) / E::G), jt = (int)((row.phase + id) % E::G);
-        const bool same = same_phase(xr, dr);
-        for (int k = threadIdx.x; k < n; k += NT) {
+            for (int k = threadIdx.x; k < n; k += NT) {
             float x[E::G];
             E::get(row.template load<true>(k), x);
 #pragma unroll
@@ -589,7 +587,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
                 for (int j = 0; j < E::G; ++j)
                     if (j == jt) x[j] += wr;
             }
-            put_granule<DT>(row, k, E::put(x), dr, same);
+            put_granule<DT>(row, k, E::put(x), dr);
         }
     }
 }

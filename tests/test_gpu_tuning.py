@@ -465,13 +465,15 @@ def test_embedding_layouts(ops):
             check_embedding(ops, i, W, 1.5, dout[:1, :1, :D].expand(*i.shape, D), None, name + " one gradient")
 
 
-def test_embedding_into_a_static_gradient_buffer(ops):
+@pytest.mark.parametrize("D,N", [(40, 60), (37, 60), (3, 900), (1, 10), (301, 900)])
+def test_embedding_into_a_static_gradient_buffer(ops, D, N):
     from bmt_amd.parallel import GradientReducer
     g = gen(6)
-    W = torch.nn.Parameter(torch.randn(300, 40, device="cuda", generator=g))
-    red = GradientReducer([W], overlap=False)
-    ids = torch.randint(0, 50, (4, 60), device="cuda", generator=g)
-    dout = torch.randn(4, 60, 40, device="cuda", generator=g)
+    other = torch.nn.Parameter(torch.zeros(3, device="cuda"))          # (the table's buffer starts behind it, at an odd element)
+    W = torch.nn.Parameter(torch.randn(300, D, device="cuda", generator=g))
+    red = GradientReducer([other, W], overlap=False)
+    ids = torch.randint(0, 50, (4, N), device="cuda", generator=g)
+    dout = torch.randn(4, N, D, device="cuda", generator=g)
     red.zero_grad()
     W.grad[7] += 3.0
     ops.embedding(ids, W, 2.0, PAD).backward(dout)
@@ -479,7 +481,7 @@ def test_embedding_into_a_static_gradient_buffer(ops):
     _, d64, absum, most = embedding64(ids, W.detach(), 2.0, dout, PAD)
     d64 *= 2
     d64[7] += 3.0
-    within(W.grad, d64, (36 + most / 4) * U * 2 * absum + 4 * U * d64.abs(), "static gradient")
+    within(W.grad, d64, (36 + most / (4 if ids.numel() <= 2048 else 32)) * U * 2 * absum + 4 * U * d64.abs(), "static gradient")
     red.remove()
 
 
