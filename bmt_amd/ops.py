@@ -2529,6 +2529,16 @@ def _ls_kl_forward(p2, t, smoothing, pad_idx, rowsum=None):
     return loss, ws
 
 
+def _settle_later(handle):
+    """the handle's parameters were counted by GeneratorFn, whose own node may not run: flush_dw settles that (once per handle)"""
+    hs = context().gen_handles
+    if any(h is handle for h in hs):
+        return
+    if len(hs) >= 8:          # (a caller that never settles them -- plain loss.backward() loops -- must not accumulate handles)
+        del hs[:-7]
+    hs.append(handle)
+
+
 class FusedGenLossFn(torch.autograd.Function):
     """LabelSmoothing(Generator(x)) as ONE autograd node over the generator's input and parameters (model/generators.py:18-19 +
     loss/label_smoothing.py:12-32): the forward reads the log-probabilities the generator already wrote (row sums + two gathers per row),
@@ -2547,10 +2557,7 @@ class FusedGenLossFn(torch.autograd.Function):
         ctx.meta = (smoothing, pad_idx, x.shape)
         ctx.params = (W, b)
         ctx.handle = handle
-        hs = context().gen_handles
-        if len(hs) >= 8:          # (a caller that never settles them -- plain loss.backward() loops -- must not accumulate handles)
-            del hs[:-7]
-        hs.append(handle)
+        _settle_later(handle)
         return loss
 
     @staticmethod
@@ -3700,6 +3707,37 @@ def _logit_grad(logits, ids, mask, pad_idx, stats_ptr, w_ptr, wb, wt, g, out=Non
     return out
 
 
+class GenLogitsFn(torch.autograd.Function):
+    """A Generator's log-probabilities as the logits of a loss from logits, as a node of its own over the generator's input and parameters: such a
+    loss takes log-softmax itself (which leaves log-probabilities as they are), its gradient sums to zero over a row, and the way back through the
+    generator's log-softmax (GeneratorFn: three passes over the (B*Tc, V) tensor) would return the same values"""
+
+    @staticmethod
+    def forward(ctx, x, W, b, handle, shape):
+        note_use(W, b)
+        xc = _f32c(x)
+        ctx.save_for_backward(xc.view(-1, xc.shape[-1]))
+        ctx.params, ctx.xshape = (W, b), x.shape
+        _settle_later(handle)
+        return handle.logp.view(shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d):
+        (x2,) = ctx.saved_tensors
+        W, b = ctx.params
+        dx, dW, db = lin_bwd(_f32c(d).view(-1, W.shape[0]), W, b, x2, need_dx=ctx.needs_input_grad[0])
+        return None if dx is None else dx.view(ctx.xshape), dW, db, None, None
+
+
+def _as_logits(pred):
+    """pred, or -- a Generator's untouched output in a pass that records a graph -- its values behind GenLogitsFn"""
+    h = getattr(pred, "_bmt_gen", None)
+    if not FUSE_GEN_LOSS or h is None or h.logp is None or not _recorded(pred) or generator_handle(pred) is None:
+        return pred
+    return GenLogitsFn.apply(h.x, h.W, h.b, h, pred.shape)
+
+
 class TokenLogpFn(torch.autograd.Function):
     """log_softmax(logits)[ids], per row; the backward recomputes the softmax from the row's maximum and sum"""
 
@@ -3728,6 +3766,7 @@ def token_logp(logits, ids, mask=None, pad_idx: Optional[int] = None):
     no gradient.  What a policy or preference loss takes as old and reference values."""
     _check_rows("token_logp", logits, ids, mask)
     _tuning_device("token_logp", logits, ids, mask)
+    logits = _as_logits(logits)
     return TokenLogpFn.apply(logits, ids, mask, pad_idx, _recorded(logits))
 
 
@@ -3816,6 +3855,7 @@ def policy_loss(logits, ids, old_logp, advantages, ref_logp=None, mask=None, pad
         raise ValueError("policy_loss: advantages are needed")
     if kl_coef != 0 and ref_logp is None:
         raise ValueError(f"policy_loss: a KL term of {kl_coef} needs ref_logp")
+    logits = _as_logits(logits)
     loss, info = PolicyLossFn.apply(logits, ids, old_logp, advantages, ref_logp, mask, pad_idx, float(clip_low), float(clip_high), float(kl_coef),
                                     _REDUCTIONS[reduction], _recorded(logits))
     return loss, PolicyStats(info, ids.shape)
@@ -3866,6 +3906,7 @@ def preference_loss(logits, ids, ref_logp, mask=None, pad_idx: Optional[int] = N
         raise ValueError(f"preference_loss: ref_logp of shape {tuple(ref_logp.shape)} and type {ref_logp.dtype} (float32 ({B},))")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"preference_loss: label_smoothing {label_smoothing}")
+    logits = _as_logits(logits)
     return PreferenceLossFn.apply(logits, ids, ref_logp, mask, pad_idx, float(beta), float(label_smoothing), bool(mean_logp), _recorded(logits))
 
 

@@ -785,3 +785,44 @@ def test_vocabulary_embedder_without_positions_uses_the_sorted_gradient(ops):
     (dW,) = torch.autograd.grad(out, W, up)
     _, d64, absum, most = embedding64(ids, W.detach(), math.sqrt(40), up, None)
     within(dW, d64, (36 + most / 4) * U * absum, "dW")
+
+
+def test_losses_behind_a_generator_skip_its_softmax(ops, monkeypatch):
+    """applied to a Generator's untouched output the losses' gradient goes straight to the generator's products: what the way through its
+    log-softmax gives, alone, beside another consumer of the same output, and not at all where the output was written to"""
+    from bmt_amd.model.generators import Generator
+    torch.manual_seed(0)
+    generator = Generator(48, 203).cuda()
+    g = gen(12)
+    x = torch.randn(3, 7, 48, device="cuda", generator=g).requires_grad_(True)
+    ids = torch.randint(2, 203, (3, 7), device="cuda", generator=g)
+    old, adv = torch.full((3, 7), -5.3, device="cuda"), torch.randn(3, device="cuda", generator=g)
+    other = torch.randn(3, 7, 203, device="cuda", generator=g) * 1e-3
+    seq = torch.zeros(2, device="cuda")
+    leaves = [x, generator.linear.weight, generator.linear.bias]
+    losses = {"policy": lambda p: ops.policy_loss(p, ids, old, adv)[0], "logp": lambda p: ops.token_logp(p, ids).square().mean(),
+              "preference": lambda p: ops.preference_loss(p.narrow(0, 0, 2), ids[:2], seq)[0]}
+    for name, loss in losses.items():
+        for extra in (False, True):
+            got = {}
+            for fused in (True, False):
+                monkeypatch.setattr(ops, "FUSE_GEN_LOSS", fused)
+                pred = generator(x)
+                total = loss(pred) + ((pred * other).sum() if extra else 0.0)
+                got[fused] = torch.autograd.grad(total, leaves)
+            for a, b in zip(got[True], got[False]):
+                # the same values up to fp32 roundings before the bf16 operand plane, where one of them moves a value by at most a step: 2^-7 of it
+                assert float((a - b).double().norm()) <= 2.0 ** -7 * float(b.double().norm()), (name, extra)
+    monkeypatch.setattr(ops, "FUSE_GEN_LOSS", True)
+    pred = generator(x)
+    calls = []
+    monkeypatch.setattr(ops.GenLogitsFn, "apply", lambda *a, f=ops.GenLogitsFn.apply: (calls.append(1), f(*a))[1])
+    ops.token_logp(pred, ids)
+    ops.token_logp(pred * 1.0, ids)
+    assert len(calls) == 1
+    ops.policy_loss(pred, ids, old, adv)
+    assert len(calls) == 2
+    with torch.no_grad():
+        assert ops.token_logp(generator(x), ids).shape == (3, 7)
+    first = torch.autograd.grad(ops.policy_loss(pred, ids, old, adv)[0] * 2.0, leaves, retain_graph=True)
+    assert all(torch.isfinite(t).all() for t in first)
