@@ -5,9 +5,12 @@
 // Two launches: `norm` leaves one 64-bit partial sum per workgroup; every workgroup of `apply` adds those (they come from L2), in one order, and
 // scales its tiles, walking them backwards: the tiles the norm read last are the ones the memory-side cache still holds.  The norm's loads are
 // ordinary ones for that reason; those and the stores of `apply` pass the caches by (nontemporal: 120 -> 97 us for 50 M fp32 values, 488 -> 424 us
-// for 335 M bf16 values into fp32; with nontemporal loads in the norm, too, 104 and 433 us).
-// Sums are 64-bit across a thread's share of a tile, and no value is lost to the range of fp32 (norm_tile).  No atomics.
-// The tensors are cut into tiles (of 32 KB: 8 loads of 16 bytes in flight per thread) by the caller's table, so a model of 200 tensors and one arena load the chip alike.
+// for 313 M bf16 values into fp32; with nontemporal loads in the norm, too, 104 and 433 us).
+// Squares and sums are 64-bit: a product of two fp32 values is exact there and cannot leave the range, and HBM leaves the time for it (fp32 squares:
+// 97.6 and 425 us, the same).  No atomics.
+// The tensors are cut into tiles (of 32 KB: 8 loads of 16 bytes in flight per thread) by the caller's table, so a model of 200 tensors and one arena
+// load the chip alike.  Measured: 50 M fp32 values 34 us for the norm (5.9 TB/s) and 63 us for reading again and writing (6.4 TB/s); 313 M bf16 values into
+// fp32 104 us (6.0 TB/s) and 320 us (5.9 TB/s).
 #include "common.h"
 
 namespace {
@@ -71,18 +74,14 @@ __device__ __forceinline__ int head_of(const char* p, int n) {
     return h < n ? h : n;
 }
 
-// A thread's share of a tile (at most 64 + 2 values).  Its squares are added in fp32 -- conversions and 64-bit products for every value took a third
-// of the time -- and that sum goes into the 64-bit one.  A sum outside [2^-80, 2^100] may have lost values to the ends of fp32's range (or is zero,
-// infinite or NaN): those shares, rare in gradients, are added again in 64 bits
-template <int DT, bool INF, bool WIDE>
-__device__ __forceinline__ void norm_share(const Tile& t, Acc& a, float& s32) {
+template <int DT, bool INF>
+__device__ __forceinline__ void norm_tile(const Tile& t, Acc& a) {
     constexpr int E = esize<DT>(), G = 16 / E, U = 8;
     const int h = head_of<DT>(t.g, t.n), nv = (t.n - h) / G, tail = h + nv * G;
     const auto v = global_at<const u32x4>(t.g, (int64_t)h * E);
     auto add = [&](float x) {
         if constexpr (INF) a.m = max(a.m, __float_as_uint(x) & 0x7fffffffu);
-        else if constexpr (WIDE) a.s = fma((double)x, (double)x, a.s);
-        else s32 = __fmaf_rn(x, x, s32);
+        else a.s = fma((double)x, (double)x, a.s);
     };
     for (int i = threadIdx.x; i < nv; i += 256 * U) {
         u32x4 q[U];
@@ -106,15 +105,6 @@ __device__ __forceinline__ void norm_share(const Tile& t, Acc& a, float& s32) {
     }
     if ((int)threadIdx.x < h) add(get1<DT>(t.g + threadIdx.x * E));
     if ((int)threadIdx.x < t.n - tail) add(get1<DT>(t.g + (int64_t)(tail + threadIdx.x) * E));
-}
-template <int DT, bool INF>
-__device__ __forceinline__ void norm_tile(const Tile& t, Acc& a) {
-    float s32 = 0.f;
-    norm_share<DT, INF, false>(t, a, s32);
-    if constexpr (!INF) {
-        if (s32 >= 0x1p-80f && s32 <= 0x1p100f) a.s += (double)s32;
-        else norm_share<DT, INF, true>(t, a, s32);
-    }
 }
 
 template <bool INF>
