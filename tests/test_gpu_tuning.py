@@ -826,3 +826,128 @@ def test_losses_behind_a_generator_skip_its_softmax(ops, monkeypatch):
         assert ops.token_logp(generator(x), ids).shape == (3, 7)
     first = torch.autograd.grad(ops.policy_loss(pred, ids, old, adv)[0] * 2.0, leaves, retain_graph=True)
     assert all(torch.isfinite(t).all() for t in first)
+
+
+# ----------------------------------------------------------------------------- beyond 32 bits, and two calls at once
+def test_logits_beyond_32_bit_offsets(ops):
+    """2.2e9 logits: the last rows against 64 bits"""
+    R, V = 66001, 33001
+    x = torch.empty(1, R, V, device="cuda", dtype=torch.bfloat16)
+    g = gen(1)
+    for part in x[0].split(8192):
+        part.copy_(torch.randn(part.shape, device="cuda", generator=g, dtype=torch.bfloat16))
+    x.requires_grad_(True)
+    ids = torch.randint(0, V, (1, R), device="cuda", generator=g)
+    mask = torch.zeros(1, R, dtype=torch.bool, device="cuda")
+    mask[0, -3:], mask[0, 100] = True, True
+    adv = torch.ones(1, device="cuda")
+    lp = logp64(x.detach()[:, -3:], ids[:, -3:])
+    loss, stats = ops.policy_loss(x, ids, None, adv, mask=mask, reduction="sum")
+    (dx,) = torch.autograd.grad(loss, x)
+    within(stats.logp[:, -3:], lp, (64 + V / 64) * U + U * lp.abs(), "logp")
+    want = torch.softmax(x.detach()[:, -3:].double(), -1)
+    want.scatter_add_(-1, ids[:, -3:, None], torch.full((1, 3, 1), -1.0, device="cuda", dtype=torch.float64))
+    tol = (256 + V / 32) * U + HALF[torch.bfloat16] * want.abs()
+    within(dx[:, -3:], want, tol, "dlogits")
+    assert int((dx[0, 101:-3].amax(1) != 0).sum()) == 0
+    d2 = torch.autograd.grad(ops.token_logp(x, ids, mask).sum(), x)[0]
+    within(d2[:, -3:], -want, tol, "token_logp's dlogits")
+
+
+def test_embedding_beyond_32_bit_offsets(ops):
+    """2.3e9 values of output and gradient"""
+    N, V, D = 280001, 40, 8200
+    g = gen(2)
+    W = torch.randn(V, D, device="cuda", generator=g).bfloat16().requires_grad_(True)
+    ids = torch.randint(0, V - 1, (N,), device="cuda", generator=g)
+    ids[-1] = V - 1          # a token that only the last position holds
+    out = ops.embedding(ids, W, 2.0)
+    assert torch.equal(out[-5:], W.detach()[ids[-5:]] * 2.0)
+    dout = torch.zeros(N, D, device="cuda", dtype=torch.bfloat16)
+    dout[-1], dout[0] = 1.0, 0.5
+    (dW,) = torch.autograd.grad(out, W, dout)
+    want = torch.zeros(V, D, device="cuda")
+    want[V - 1] += 2.0
+    want[ids[0]] += 1.0
+    assert torch.equal(dW.float(), want)
+
+
+def test_a_gradient_beyond_32_bit_offsets():
+    from bmt_amd.optim import GradClipper
+    n = 2 ** 31 + 12345
+    t = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    t[-1], t[0], t[n // 2] = 4.0, 2.0, 4.0
+    assert float(GradClipper([t], 3.0)()) == 6.0
+    assert [float(t[i]) for i in (0, n // 2, n - 1)] == [1.0, 2.0, 2.0] and float(t[1:5].abs().sum()) == 0.0
+
+
+def test_many_rows_of_few_tokens(ops):
+    """a million rows: several adding and counting workgroups"""
+    B, T, V = 1000, 1003, 6
+    g = gen(3)
+    x = torch.randn(B, T, V, device="cuda", generator=g).requires_grad_(True)
+    ids = torch.randint(0, V, (B, T), device="cuda", generator=g)
+    mask = torch.rand(B, T, device="cuda", generator=g) > 0.5
+    old, adv = torch.full((B, T), -2.0, device="cuda"), torch.randn(B, device="cuda", generator=g)
+    for reduction in ("token", "sequence"):
+        loss, stats = ops.policy_loss(x, ids, old, adv, old - 0.1, mask, kl_coef=0.1, reduction=reduction)
+        (dx,) = torch.autograd.grad(loss, x)
+        x64 = x.detach().double().requires_grad_(True)
+        want, kl, clipped = policy64(logp64(x64, ids), old, adv, old - 0.1, mask, beta=0.1, reduction=reduction)
+        (d64,) = torch.autograd.grad(want, x64)
+        # (ratios up to e^2 here; rows whose ratio is at a border to rounding: none may differ by more than its own size, and few do)
+        near = (dx.double() - d64).abs() > (256 + V / 32) * U * 16 * float(d64.abs().max())
+        assert int(near.any(-1).sum()) <= 20
+        within(loss, want, 1e-6 * float(adv.abs().max()), "loss")
+        within(stats.kl, kl, 16 * 64 * U, "kl")
+        within(stats.clip_fraction, clipped, 20 / float(mask.sum()) + U, "clip fraction")
+
+
+def test_calls_at_once_on_two_streams(ops):
+    """independent calls issued alternately on two streams, and from two threads: each has the result it has alone"""
+    import threading
+    from bmt_amd.optim import GradClipper
+    g = gen(8)
+    V, B, T = 5003, 6, 40
+    xs = [torch.randn(B, T, V, device="cuda", generator=g).requires_grad_(True) for _ in range(2)]
+    ids = [torch.randint(0, V, (B, T), device="cuda", generator=g) for _ in range(2)]
+    rows = [torch.full((B, T), -9.0, device="cuda") + torch.randn(B, T, device="cuda", generator=g) for _ in range(2)]
+    Ws = [torch.randn(V, 64, device="cuda", generator=g).requires_grad_(True) for _ in range(2)]
+    ups = [torch.randn(B, T, 64, device="cuda", generator=g) for _ in range(2)]
+    grads = [[torch.randn(100000, device="cuda", generator=g) for _ in range(5)] for _ in range(2)]
+    outs = [[torch.empty_like(t) for t in ts] for ts in grads]
+    clips = [GradClipper(a, 0.5, b) for a, b in zip(grads, outs)]
+
+    def work(k):
+        loss, _ = ops.policy_loss(xs[k], ids[k], rows[k], rows[k][:, 0], rows[k], kl_coef=0.1)
+        (dx,) = torch.autograd.grad(loss, xs[k])
+        pl, r = ops.preference_loss(xs[k], ids[k], rows[k][:, 1])
+        (dp,) = torch.autograd.grad(pl, xs[k])
+        (dW,) = torch.autograd.grad(ops.embedding(ids[k], Ws[k], 3.0), Ws[k], ups[k])
+        return [loss.detach(), dx, pl.detach(), r, dp, dW, clips[k](), outs[k][4].clone()]
+
+    alone = [work(k) for k in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(work(k))
+    torch.cuda.synchronize()
+
+    def loop(k):
+        with torch.cuda.stream(streams[k]):
+            for _ in range(5):
+                got[k].append(work(k))
+            streams[k].synchronize()
+    threads = [threading.Thread(target=loop, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert len(got[k]) == 10
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, alone[k]))
