@@ -9,8 +9,8 @@
 // Numerics: maxima and exponentials in fp32, a thread's partial sums in fp32 (at most a few hundred terms), across threads and everything that
 // belongs to a row or a sequence in 64 bits; 16-bit gradients are rounded once.  No atomics: results do not depend on the schedule.
 // Rows that do not count (mask 0, or the padding id) are not read; their gradient rows are written as zeros.
-// Measured: policy loss with its gradient, all rows counting, 8192 x 32000 bf16 207 us (5.1 TB/s of logits read + gradients written; a plain copy
-// reaches 5.95), 65536 x 1000 bf16 80 us; preference loss 16 x 1024 x 32000 bf16, a third of the rows masked: 126 us for the log-probabilities (5.5 TB/s
+// Measured: policy loss with its gradient, all rows counting, 8192 x 32000 bf16 202 us (5.2 TB/s of logits read + gradients written; a plain copy
+// reaches 5.95), 65536 x 1000 bf16 78 us; preference loss 16 x 1024 x 32000 bf16, a third of the rows masked: 121 us for the log-probabilities (5.7 TB/s
 // of the rows read), 292 us for the gradient (5.9 TB/s).
 #include "common.h"
 
@@ -79,6 +79,9 @@ constexpr double EXP_BIAS = 3.3e-9;
 __device__ __forceinline__ float exp_neg(float t) {
     return __builtin_amdgcn_exp2f(__fmaf_rn(t, 1.44269502162933349609375f, t * 1.92596299112661746e-8f));
 }
+// for gradients: log2 e as one float (1.3e-8 |t| off, below their own rounding)
+__device__ __forceinline__ float exp_grad(float t) { return __builtin_amdgcn_exp2f(t * 1.44269502162933349609375f); }
+
 // the (B, T) rows of a call: logits with two row strides, ids and an optional mask with theirs (all strides in elements)
 struct Rows {
     const char* x;
@@ -318,6 +321,13 @@ __global__ __launch_bounds__(256) void count_rows_kernel(Rows q, int B, int per_
     if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
+// the granules as they were loaded, to be taken apart again: left alone the compiler keeps the floats of one use for the next (twice the registers)
+template <int NV>
+__device__ __forceinline__ void only_raw(u32x4 (&v)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i]));
+}
+
 // ---------------------------------------------------------------- forward: statistics and log-probability of every row, any V
 // One sweep with a running maximum and sum per thread.  stats[r] = {max, 1 / sum} for the gradient kernel (0, 0 where the row does not count).
 template <int DT, int NT, bool POLICY>
@@ -329,7 +339,7 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
     __shared__ double redd[NT / 64];
     __shared__ int redi[NT / 64];
     const int64_t r = blockIdx.x;
-    const int b = (int)(r / q.T), t = (int)(r % q.T);
+    const int b = (int)(blockIdx.x / (unsigned)q.T), t = (int)(blockIdx.x % (unsigned)q.T);
     const int64_t id = q.id[b * q.ib + t * q.it];
     if (!row_counts(q, b, t, id)) {
         if (threadIdx.x == 0) {
@@ -361,7 +371,8 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
     const float spread = (float)((((uint32_t)r * 0x9E3779B1u) ^ (threadIdx.x * 0x85EBCA6Bu)) >> 20) * 0x1p-12f;
     float m = -__builtin_huge_valf(), ms = 0.f;
     double s = 0.0;
-    for (int k0 = threadIdx.x; k0 < n; k0 += NT * U) {
+    for (int k1 = 0; k1 < n; k1 += NT * U) {
+        const int k0 = k1 + threadIdx.x;
         u32x4 v[U];
         const uint32_t l = E::lowest();
 #pragma unroll
@@ -383,8 +394,10 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
         float a = 0.f;
 #pragma unroll
         for (int i = 0; i < U; ++i)
+            if (k1 + i * NT < n) {      // (whole slots behind the row's end)
 #pragma unroll
-            for (int j = 0; j < E::G; ++j) a += exp_neg(x[i][j] - ms);
+                for (int j = 0; j < E::G; ++j) a += exp_neg(x[i][j] - ms);
+            }
         s += (double)a;
     }
     double norm = 1.0;
@@ -406,13 +419,6 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
     }
 }
 
-// the granules as they were loaded, to be taken apart again: left alone the compiler keeps the floats of one use for the next (twice the registers)
-template <int NV>
-__device__ __forceinline__ void only_raw(u32x4 (&v)[NV]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i]));
-}
-
 // ---------------------------------------------------------------- policy loss: statistics, loss terms and gradient of a row in one visit
 // The row (at most NT * NV granules) stays in registers as it was loaded.
 template <int DT, int NT, int NV>
@@ -424,7 +430,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     __shared__ int redi[NT / 64];
     __shared__ float wc[2];
     const int64_t r = blockIdx.x;
-    const int b = (int)(r / q.T), t = (int)(r % q.T);
+    const int b = (int)(blockIdx.x / (unsigned)q.T), t = (int)(blockIdx.x % (unsigned)q.T);
     const int64_t id = q.id[b * q.ib + t * q.it];
     const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
     char* dr = dx + (b * db + t * dt) * E::B;
@@ -500,7 +506,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
             float x[E::G];
             E::get(v[i], x);
 #pragma unroll
-            for (int j = 0; j < E::G; ++j) x[j] = exp_neg(x[j] - m) * c;
+            for (int j = 0; j < E::G; ++j) x[j] = exp_grad(x[j] - m) * c;
             if (k == kt) {
 #pragma unroll
                 for (int j = 0; j < E::G; ++j)
@@ -566,7 +572,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
     if (once && gs == 1.f) return;
     for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
         const int64_t r = rows - 1 - i;      // last rows first: what the forward pass read last is what the memory-side cache still holds
-        const int b = (int)(r / q.T), t = (int)(r % q.T);
+        const int b = (int)((unsigned)r / (unsigned)q.T), t = (int)((unsigned)r % (unsigned)q.T);
         const int64_t id = q.id[b * q.ib + t * q.it];
         const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
         char* dr = dx + (b * db + t * dt) * E::B;
@@ -584,7 +590,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
             float x[E::G];
             E::get(row.template load<true>(k), x);
 #pragma unroll
-            for (int j = 0; j < E::G; ++j) x[j] = exp_neg(x[j] - m) * c;
+            for (int j = 0; j < E::G; ++j) x[j] = exp_grad(x[j] - m) * c;
             if (k == kt) {
 #pragma unroll
                 for (int j = 0; j < E::G; ++j)
@@ -596,9 +602,6 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
 }
 
 // ---------------------------------------------------------------- preference loss from the rows' log-probabilities: a wave per pair
-__device__ __forceinline__ double softplus64(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
-__device__ __forceinline__ double sigmoid64(double x) { return 1.0 / (1.0 + exp(-x)); }
-
 constexpr int PAIRS_WG = 128;      // most pairs of one workgroup (their sums stand in LDS)
 
 // workgroup g: pairs [g * each, ..).  A wave adds up a sequence, then a thread works out a pair.  gridDim.x == 1: loss[0], else part[g] (sum_f64_kernel)
@@ -607,20 +610,43 @@ __global__ __launch_bounds__(1024) void preference_pairs_kernel(const double* __
                                                                  double* __restrict__ part, float* __restrict__ loss) {
     __shared__ double sum[2][PAIRS_WG], len[2][PAIRS_WG], red[16];
     const int lane = threadIdx.x & 63, p0 = blockIdx.x * each, n = min(each, P - p0);
-    for (int j = threadIdx.x >> 6; j < 2 * n; j += 16) {
-        const int h = j >= n, i = j - h * n;
-        const int64_t r0 = (int64_t)(p0 + i + h * P) * T;
-        double a = 0.0, c = 0.0;
-#pragma unroll 4
-        for (int t = lane; t < T; t += 64) {
-            a += logp[r0 + t];
-            if (mean) c += stats[r0 + t].y == 0.f ? 0.0 : 1.0;      // (a row that counts has a finite sum)
-        }
+    float ref0 = 0.f, ref1 = 0.f;      // (on their way beside the sums)
+    if ((int)threadIdx.x < n) {
+        ref0 = ref[(int64_t)(p0 + threadIdx.x) * rs];
+        ref1 = ref[(int64_t)(p0 + threadIdx.x + P) * rs];
+    }
+    auto keep = [&](int j, double a, double c) {
         a = wave_sum_f64(a);
         c = wave_sum_f64(c);
         if (lane == 0) {
-            sum[h][i] = a;
-            len[h][i] = mean ? fmax(c, 1.0) : 1.0;
+            sum[j >= n][j >= n ? j - n : j] = a;
+            len[j >= n][j >= n ? j - n : j] = mean ? fmax(c, 1.0) : 1.0;
+        }
+    };
+    auto row = [&](int j, int t) { return (int64_t)(p0 + (j >= n ? j - n + P : j)) * T + t; };
+    auto counts = [&](int64_t r) { return !mean || stats[r].y == 0.f ? 0.0 : 1.0; };      // (a row that counts has a finite sum)
+    if (T <= 64) {      // short sequences, four of a wave's at a time: their loads are on their way together
+        for (int j0 = threadIdx.x >> 6; j0 < 2 * n; j0 += 64) {
+            double a[4] = {}, c[4] = {};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (j0 + 16 * k < 2 * n && lane < T) {
+                    a[k] = logp[row(j0 + 16 * k, lane)];
+                    c[k] = counts(row(j0 + 16 * k, lane));
+                }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (j0 + 16 * k < 2 * n) keep(j0 + 16 * k, a[k], c[k]);
+        }
+    } else {
+        for (int j = threadIdx.x >> 6; j < 2 * n; j += 16) {
+            double a = 0.0, c = 0.0;
+#pragma unroll 4
+            for (int t = lane; t < T; t += 64) {
+                a += logp[row(j, t)];
+                c += counts(row(j, t));
+            }
+            keep(j, a, c);
         }
     }
     __syncthreads();
@@ -628,13 +654,15 @@ __global__ __launch_bounds__(1024) void preference_pairs_kernel(const double* __
     if ((int)threadIdx.x < n) {
         const int i = threadIdx.x, g = p0 + i;
         const double i0 = 1.0 / len[0][i], i1 = 1.0 / len[1][i];
-        const double r0 = (double)beta * (sum[0][i] * i0 - (double)ref[(int64_t)g * rs]), r1 = (double)beta * (sum[1][i] * i1 - (double)ref[(int64_t)(g + P) * rs]);
+        const double r0 = (double)beta * (sum[0][i] * i0 - (double)ref0), r1 = (double)beta * (sum[1][i] * i1 - (double)ref1);
         const double z = r0 - r1, ls = (double)smoothing;
-        l = (1.0 - ls) * softplus64(-z);
-        double d = (1.0 - ls) * sigmoid64(-z);
+        // log sigmoid and sigmoid of both signs from one exponential: e = e^-|z|
+        const double e = exp(-fabs(z)), rest = log1p(e), one = 1.0 / (1.0 + e), up = z >= 0.0 ? e * one : one;      // up = sigmoid(-z)
+        l = (1.0 - ls) * (fmax(-z, 0.0) + rest);
+        double d = (1.0 - ls) * up;
         if (ls != 0.0) {      // (0 * inf)
-            l += ls * softplus64(z);
-            d -= ls * sigmoid64(z);
+            l += ls * (fmax(z, 0.0) + rest);
+            d -= ls * (z >= 0.0 ? one : e * one);
         }
         l /= (double)P;
         d *= -(double)beta / (double)P;
