@@ -35,6 +35,11 @@ struct Split {
 };
 
 __device__ __forceinline__ int clamp_id(int64_t id, int V) { return id < 0 ? 0 : (id >= V ? V - 1 : (int)id); }
+// the token whose gradient a position adds to, -1: none (the padding id, and ids that are clamped to it)
+__device__ __forceinline__ int grad_token(int64_t id, int V, int64_t pad) {
+    const int v = clamp_id(id, V);
+    return id == pad || v == pad ? -1 : v;
+}
 
 template <int BYTES>
 struct Vec;
@@ -144,9 +149,8 @@ __global__ __launch_bounds__(1024) void embed_order_kernel(const int64_t* __rest
     auto fetch = [&](int64_t n) -> int {
         if (n >= last) return -2;
         if constexpr (K < 0) return sp.key[n];
-        const int64_t id = ids[n];
-        const int v = clamp_id(id, V), o = v & gmask;
-        return id == pad || o > me ? -2 : (o < me ? -1 : v >> ow.lg);
+        const int v = grad_token(ids[n], V, pad), o = v & gmask;
+        return v < 0 || o > me ? -2 : (o < me ? -1 : v >> ow.lg);
     };
     auto count = [&](int k) {
         if (k == -1) ++below;
@@ -232,8 +236,8 @@ __global__ __launch_bounds__(1024) void embed_count_kernel(const int64_t* __rest
     for (int i = 0; i < R; ++i) {
         const int64_t n = ((int64_t)blockIdx.x * R + i) * 1024 + threadIdx.x;
         if (n < N) {
-            const int64_t id = ids[n];
-            if (id != pad) atomicAdd(&hist[clamp_id(id, V) & (G - 1)], 1);
+            const int v = grad_token(ids[n], V, pad);
+            if (v >= 0) atomicAdd(&hist[v & (G - 1)], 1);
         }
     }
     __syncthreads();
@@ -260,9 +264,7 @@ __global__ __launch_bounds__(1024) void embed_split_kernel(const int64_t* __rest
     const int64_t first = ((int64_t)me * 16 + wave) * 64 * R;
     int* mine = hist + wave * G;
     auto fetch = [&](int64_t n) -> int {
-        if (n >= N) return -1;
-        const int64_t id = ids[n];
-        return id == pad ? -1 : clamp_id(id, V);
+        return n < N ? grad_token(ids[n], V, pad) : -1;
     };
     for (int i = 0; i < R; ++i) {
         const int v = fetch(first + i * 64 + lane);
@@ -475,6 +477,8 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__
     if (wave == 0 && in) finish_row<DT, G>(dW, into, ldw, ow.token(u), c, D, scale, acc[0]);
 }
 
+constexpr int64_t MAX_GRID = 0xffffffff / 256;      // workgroups of 256 threads
+
 inline int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 inline int64_t emb_ld(int D) { return (D + 7) / 8 * 8; }      // floats per partial sum: 16-byte rows for every G
 
@@ -489,8 +493,8 @@ inline Owners owners_for(int V) {
     return ow;
 }
 inline bool splits(int64_t N, const Owners& ow) { return N > EMB_DIRECT && (1 << ow.lg) <= EMB_SPLIT_G; }
-// ids per thread and chunk of the split: at most 256 chunks up to 4 M ids (every workgroup adds up the counts of all chunks)
-inline int split_rounds(int64_t N) { return N <= 256 * 1024 ? 1 : N <= 1024 * 1024 ? 4 : 16; }
+// ids per thread and chunk of the split: at most 256 chunks up to 4 M ids and 1024 beyond (every workgroup adds up the counts of all chunks)
+inline int split_rounds(int64_t N) { return N <= 256 * 1024 ? 1 : N <= 1024 * 1024 ? 4 : N <= 16 * 1024 * 1024 ? 16 : (int)((N + 1024 * 1024 - 1) / (1024 * 1024)); }
 inline int64_t split_chunks(int64_t N) { return (N + 1024 * split_rounds(N) - 1) / (1024 * split_rounds(N)); }
 inline int groups_for(const Owners& ow, int V) { return V < (1 << ow.lg) ? V : 1 << ow.lg; }
 
@@ -520,7 +524,7 @@ extern "C" int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, voi
     const int es = dtype == BMT_DT_F32 ? 4 : 2, g = cols_of(es, D), ncb = bmt_cdiv(D, 64 * g);
     const int tpw = N >= 16384 ? 4 : 1;      // enough waves to fill the chip: four tokens' loads in flight in each
     const int64_t tasks = (N + tpw - 1) / tpw * ncb, grid = (tasks + 3) / 4;
-    BMT_CHECK_ARG(grid <= 0x7fffffff, "bmt_embedding: too many tokens");
+    BMT_CHECK_ARG(grid <= MAX_GRID, "bmt_embedding: %lld tokens of %d columns are more than a grid holds", (long long)N, D);
 #define BMT_CALL(DT, G)                                                                                                                                       \
     do {                                                                                                                                                      \
         if (tpw == 4) hipLaunchKernelGGL((embed_kernel<DT, G, 4>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, ids, (const char*)W, ldw, (char*)out, N, D, V, \
@@ -566,7 +570,7 @@ extern "C" int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t l
     const int64_t chunks = N > EMB_FEW ? (N + EMB_LONG - 1) / EMB_LONG : 0;
     const int64_t grid = chunks * ncs + ((int64_t)V * ncs + 3) / 4;
     const int64_t ldp = emb_ld(D);
-    BMT_CHECK_ARG(grid <= 0x7fffffff, "bmt_embedding_bwd: vocabulary too large");
+    BMT_CHECK_ARG(grid <= MAX_GRID && chunks * ncb <= MAX_GRID, "bmt_embedding_bwd: a table of %d x %d is more than a grid holds", V, D);
     const size_t lds = (size_t)16 * ow.nb * sizeof(int);
     int bits = 0;
     while ((1 << bits) < ow.nb) ++bits;

@@ -279,8 +279,10 @@ __device__ __forceinline__ float policy_row(const PolicyIn& p, const RowIn& in, 
     if (p.ref) {
         const double d = (double)in.ref - lp;
         kl = exp_rest(d);
-        loss += (double)p.beta * kl;
-        w -= (double)p.beta * (kl + d);
+        if (p.beta != 0.f) {      // (a term that is only watched may be infinite: 0 * inf)
+            loss += (double)p.beta * kl;
+            w -= (double)p.beta * (kl + d);
+        }
     }
     *terms = Terms{loss * norm, (float)kl, clipped ? 3 : 1};
     return (float)(w * norm);
@@ -586,7 +588,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
         const float2 st = stats[r];
         const float wr = w[b * wb + t * wt] * gs, m = st.x, c = -wr * st.y;
         const int kt = (int)((row.phase + id) / E::G), jt = (int)((row.phase + id) % E::G);
-            for (int k = threadIdx.x; k < n; k += NT) {
+        for (int k = threadIdx.x; k < n; k += NT) {
             float x[E::G];
             E::get(row.template load<true>(k), x);
 #pragma unroll
@@ -658,9 +660,12 @@ __global__ __launch_bounds__(1024) void preference_pairs_kernel(const double* __
         const double z = r0 - r1, ls = (double)smoothing;
         // log sigmoid and sigmoid of both signs from one exponential: e = e^-|z|
         const double e = exp(-fabs(z)), rest = log1p(e), one = 1.0 / (1.0 + e), up = z >= 0.0 ? e * one : one;      // up = sigmoid(-z)
-        l = (1.0 - ls) * (fmax(-z, 0.0) + rest);
-        double d = (1.0 - ls) * up;
-        if (ls != 0.0) {      // (0 * inf)
+        double d = 0.0;
+        if (ls != 1.0) {      // (0 * inf, here and below)
+            l = (1.0 - ls) * (fmax(-z, 0.0) + rest);
+            d = (1.0 - ls) * up;
+        }
+        if (ls != 0.0) {
             l += ls * (fmax(z, 0.0) + rest);
             d -= ls * (z >= 0.0 ? one : e * one);
         }
@@ -688,15 +693,6 @@ __global__ __launch_bounds__(1024) void sum_f64_kernel(const double* __restrict_
 
 inline int elem_bytes(int dtype) { return dtype == BMT_DT_F32 ? 4 : 2; }
 
-int check_rows(const char* who, const void* x, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* id) {
-    BMT_CHECK_ARG(dtype == BMT_DT_F32 || dtype == BMT_DT_BF16 || dtype == BMT_DT_F16, "%s: unknown dtype %d", who, dtype);
-    BMT_CHECK_ARG(B >= 0 && T >= 0 && V > 0 && V <= (1 << 30) && sb >= 0 && st >= 0, "%s: bad sizes B=%d T=%d V=%d", who, B, T, V);
-    BMT_CHECK_ARG((int64_t)B * T <= 0x7fffffff, "%s: %d x %d rows are more than a grid holds", who, B, T);
-    BMT_CHECK_ARG((x && id) || (int64_t)B * T == 0, "%s: null pointer", who);
-    BMT_CHECK_ARG((reinterpret_cast<uintptr_t>(x) & (elem_bytes(dtype) - 1)) == 0, "%s: logits are not aligned to their elements", who);
-    return BMT_OK;
-}
-
 // threads per row: about 4 granules each are in flight in one batch, and a few rows cannot fill 256 CUs with small workgroups
 inline int threads_for(int64_t rows, int64_t granules) {
     if (granules <= 256) return 64;
@@ -704,6 +700,16 @@ inline int threads_for(int64_t rows, int64_t granules) {
 }
 
 inline int64_t granules_of(int V, int dtype) { return ((int64_t)V * elem_bytes(dtype) + 15) / 16; }
+
+int check_rows(const char* who, const void* x, int dtype, int64_t sb, int64_t st, int B, int T, int V, const int64_t* id) {
+    BMT_CHECK_ARG(dtype == BMT_DT_F32 || dtype == BMT_DT_BF16 || dtype == BMT_DT_F16, "%s: unknown dtype %d", who, dtype);
+    BMT_CHECK_ARG(B >= 0 && T >= 0 && V > 0 && V <= (1 << 30) && sb >= 0 && st >= 0, "%s: bad sizes B=%d T=%d V=%d", who, B, T, V);
+    const int64_t rows = (int64_t)B * T;
+    BMT_CHECK_ARG(rows <= 0x7fffffff && rows * threads_for(rows, granules_of(V, dtype)) <= 0xffffffff, "%s: %d x %d rows are more than a grid holds", who, B, T);
+    BMT_CHECK_ARG((x && id) || rows == 0, "%s: null pointer", who);
+    BMT_CHECK_ARG((reinterpret_cast<uintptr_t>(x) & (elem_bytes(dtype) - 1)) == 0, "%s: logits are not aligned to their elements", who);
+    return BMT_OK;
+}
 
 template <int DT>
 void launch_logp(const Rows& q, const PolicyIn* p, float* logp, double* logp64, float2* stats, float* w, Terms* terms, int64_t rows, hipStream_t st) {

@@ -3913,7 +3913,7 @@ def preference_loss(logits, ids, ref_logp, mask=None, pad_idx: Optional[int] = N
 def _embedding_forward(idc, W, scale):
     V, D = W.shape
     out = torch.empty(*idc.shape, D, device=W.device, dtype=W.dtype)
-    _run_on(W.device, "bmt_embedding", lib.bmt_embedding, idc.data_ptr(), W.data_ptr(), W.stride(0), out.data_ptr(), idc.numel(), D, V, _DTYPES[W.dtype], scale)
+    _run_on(W.device, "bmt_embedding", lib.bmt_embedding, idc.data_ptr(), W.data_ptr(), W.stride(0) if V > 1 else D, out.data_ptr(), idc.numel(), D, V, _DTYPES[W.dtype], scale)
     return out
 
 
@@ -3956,7 +3956,7 @@ class EmbeddingFn(torch.autograd.Function):
 def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
     """scale * weight[ids] (ids int64 of any shape; weight (V, D) fp32, bf16 or fp16; ids outside the table are clamped, as EmbedFn does).  The
     gradient of ``weight`` is added in fp32 over a token's positions in ascending order and rounded once -- the same bits on every run, whichever
-    tokens repeat --; ``pad_idx`` gets none.  A parameter with a static gradient buffer (GradientReducer) has it added there directly."""
+    tokens repeat --; ``pad_idx`` and ids that are clamped to it get none.  A parameter with a static gradient buffer (GradientReducer) has it added there directly."""
     _tuning_device("embedding", ids, weight)
     if weight.dim() != 2 or weight.dtype not in _DTYPES or not 0 < weight.shape[0] <= 1 << 30 or weight.shape[1] == 0:
         raise ValueError(f"embedding: a weight of shape {tuple(weight.shape)} and type {weight.dtype} (2-D float32, bfloat16 or float16)")
@@ -3964,7 +3964,7 @@ def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
         raise ValueError(f"embedding: ids of type {ids.dtype} (int64)")
     if ids.numel() > 0x7fffffff - 64:
         raise ValueError(f"embedding: {ids.numel()} ids")
-    if weight.stride(0) < weight.shape[1] or (weight.shape[1] > 1 and weight.stride(1) != 1):
+    if (weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]) or (weight.shape[1] > 1 and weight.stride(1) != 1):
         weight = weight.contiguous()
     idc = ids.contiguous()
     if _recorded(weight):

@@ -663,9 +663,9 @@ int bmt_preference_loss(const void* logits, int dtype, int64_t sb, int64_t st, i
  * bmt_prep_embed */
 int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, void* out, int64_t N, int D, int V, int dtype, float scale, void* stream);
 /* its gradient, the same bits on every run: row v = scale * sum of dout[n] over the positions n with ids[n] == v, added in fp32 in ascending
- * order of n; positions that hold pad_idx are left out (INT64_MIN: none).  dW ([V][D] at stride ldw, `dtype`): every row is written, zeros
- * where a token does not occur -- or into (fp32): the rows of the tokens that occur are added to it.  ws: bmt_embedding_bwd_ws_bytes, 16-byte
- * aligned */
+ * order of n; positions that hold pad_idx, or are clamped to it, are left out (INT64_MIN: none).  dW ([V][D] at stride ldw, `dtype`): every
+ * row is written, zeros where a token does not occur -- or into (fp32): the rows of the tokens that occur are added to it.  ws:
+ * bmt_embedding_bwd_ws_bytes, 16-byte aligned */
 int64_t bmt_embedding_bwd_ws_bytes(int64_t N, int D, int V);
 int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t ld, int64_t N, int D, int V, int dtype, float scale, int64_t pad_idx, void* dW,
                       float* into, int64_t ldw, void* ws, int64_t ws_bytes, void* stream);

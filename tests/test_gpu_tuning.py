@@ -951,3 +951,67 @@ def test_calls_at_once_on_two_streams(ops):
         assert len(got[k]) == 10
         for r in got[k]:
             assert all(torch.equal(a, b) for a, b in zip(r, alone[k]))
+
+
+# ----------------------------------------------------------------------------- calls at the edges of what the documentation allows
+def test_a_kl_term_that_is_only_watched_may_be_infinite(ops):
+    """kl_coef 0 with a reference: its KL term is a number to look at, and tokens that the reference rules out leave loss and gradient alone"""
+    g = gen(21)
+    x = torch.randn(2, 3, 40, device="cuda", generator=g).requires_grad_(True)
+    ids = torch.randint(0, 40, (2, 3), device="cuda", generator=g)
+    adv = torch.randn(2, device="cuda", generator=g)
+    ref = torch.full((2, 3), -2.0, device="cuda")
+    ref[1, 1] = -float("inf")
+    old = logp64(x.detach(), ids).float()
+    loss, stats = ops.policy_loss(x, ids, old, adv, ref)
+    (dx,) = torch.autograd.grad(loss, x)
+    alone = ops.policy_loss(x, ids, old, adv)[0]
+    assert torch.equal(loss, alone) and torch.equal(dx, torch.autograd.grad(alone, x)[0]) and bool(torch.isfinite(dx).all())
+    assert float(stats.kl) == float("inf")
+
+
+def test_preference_labels_that_are_all_wrong(ops):
+    """label_smoothing 1: only -log sigmoid(-z) counts, which is 0 where the first caption is impossible"""
+    x = torch.zeros(2, 1, 50, device="cuda")
+    x[0, 0, 7] = -float("inf")
+    ids = torch.full((2, 1), 7, device="cuda")
+    x.requires_grad_(True)
+    loss, _ = ops.preference_loss(x, ids, torch.zeros(2, device="cuda"), label_smoothing=1.0)
+    (dx,) = torch.autograd.grad(loss, x)
+    assert float(loss) == 0.0 and bool((dx == 0).all())
+
+
+@pytest.mark.parametrize("n", [40, 5000, 20000])      # (ids in registers, ids split by owner first)
+def test_ids_that_are_clamped_to_the_padding_row_add_nothing_to_it(ops, n):
+    V, D, g = 30, 8, gen(n)
+    ids = torch.randint(-9, V + 9, (n,), device="cuda", generator=g)
+    W = torch.randn(V, D, device="cuda", generator=g).requires_grad_(True)
+    dout = torch.randint(-3, 4, (n, D), device="cuda", generator=g).float()      # (sums of small integers: exact)
+    for pad in (0, V - 1, -4):
+        (dW,) = torch.autograd.grad(ops.embedding(ids, W, 1.0, pad), W, dout)
+        at = ids.clamp(0, V - 1)
+        keep = (ids != pad) & (at != pad)
+        want = torch.zeros(V, D, device="cuda").index_add_(0, at[keep], dout[keep])
+        assert torch.equal(dW, want), pad
+
+
+def test_a_table_of_one_row_in_any_layout(ops):
+    W = torch.randn(6, 1, device="cuda").t()          # (1, 6), strides (1, 1)
+    W.requires_grad_(True)
+    ids = torch.zeros(3, dtype=torch.int64, device="cuda")
+    out = ops.embedding(ids, W)
+    (dW,) = torch.autograd.grad(out, W, torch.ones_like(out))
+    assert torch.equal(out, W.detach().expand(3, 6)) and bool((dW == 3).all())
+
+
+def test_embedding_of_more_ids_than_short_chunks_hold(ops):
+    """over 16 M positions the chunks of the split grow"""
+    g = gen(3)
+    V, D, n = 1000, 4, (1 << 24) + 100001
+    ids = torch.randint(0, V, (n,), device="cuda", generator=g)
+    dout = torch.randint(-1, 2, (n, D), device="cuda", generator=g).float()      # (a token's sum stays far below 2^24: exact)
+    W = torch.randn(V, D, device="cuda", generator=g).requires_grad_(True)
+    (dW,) = torch.autograd.grad(ops.embedding(ids, W, 1.0, PAD), W, dout)
+    want = torch.zeros(V, D, device="cuda", dtype=torch.float64).index_add_(0, ids, dout.double())
+    want[PAD] = 0
+    assert torch.equal(dW.double(), want)

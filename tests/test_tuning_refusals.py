@@ -90,3 +90,16 @@ def test_gradient_layouts_are_dense_or_refused():
     t = torch.zeros(4, 6)
     assert _dense(t) and _dense(t.t()) and _dense(t[1:3]) and _dense(torch.zeros(())) and _dense(torch.zeros(2, 3, 4).permute(2, 0, 1)) and _dense(t[:, :1][:1])
     assert not _dense(t[:, :3]) and not _dense(t[::2]) and not _dense(torch.zeros(1, 6).expand(4, 6))
+
+
+def test_calls_that_no_grid_holds_are_refused():
+    """a launch has fewer than 2^32 threads: 64 for a short row, 256 for four tokens of a lookup or of a table"""
+    from bmt_amd import _lib
+    lib = _lib.load()
+    some = 4096
+    assert lib.bmt_logp_rows(some, 0, 5 << 13, 5, 1 << 14, 1 << 13, 5, some, 1 << 13, 1, None, 0, 0, -1, some, some, None) == -1
+    assert b"more than a grid holds" in lib.bmt_last_error()
+    assert lib.bmt_embedding(some, some, 64, some, 1 << 31, 64, 1000, 0, 1.0, None) == -1 and b"more than a grid holds" in lib.bmt_last_error()
+    V = 1 << 30
+    n = lib.bmt_embedding_bwd_ws_bytes(100, 6, V)
+    assert lib.bmt_embedding_bwd(some, some, 6, 100, 6, V, 0, 1.0, -1, some, None, 6, some, n, None) == -1 and b"more than a grid holds" in lib.bmt_last_error()
