@@ -6,8 +6,8 @@
 // Bound: HBM -- about 15 fp32 operations per logit against 4 - 8 bytes moved.  The policy loss needs nothing from other rows but their count, so
 // a row stays in the registers of its workgroup from the maximum to the gradient: every logit is read once and every gradient written once.  The
 // preference loss needs the whole pair before any gradient: its logits are read twice.
-// Numerics: maxima and exponentials in fp32, a thread's partial sums in fp32 (at most a few hundred terms), across threads and everything that
-// belongs to a row or a sequence in 64 bits; 16-bit gradients are rounded once.  No atomics: results do not depend on the schedule.
+// Numerics: maxima and exponentials in fp32, the sum of 16 bytes' exponentials in fp32, all other sums and everything that belongs to a row or a
+// sequence in 64 bits; 16-bit gradients are rounded once.  No atomics: results do not depend on the schedule.
 // Rows that do not count (mask 0, or the padding id) are not read; their gradient rows are written as zeros.
 // Measured: policy loss with its gradient, all rows counting, 8192 x 32000 bf16 202 us (5.2 TB/s of logits read + gradients written; a plain copy
 // reaches 5.95), 65536 x 1000 bf16 78 us; preference loss 16 x 1024 x 32000 bf16, a third of the rows masked: 121 us for the log-probabilities (5.7 TB/s
@@ -78,6 +78,18 @@ struct Elem<BMT_DT_F16> {
 constexpr double EXP_BIAS = 3.3e-9;
 __device__ __forceinline__ float exp_neg(float t) {
     return __builtin_amdgcn_exp2f(__fmaf_rn(t, 1.44269502162933349609375f, t * 1.92596299112661746e-8f));
+}
+// the sum of a granule's exponentials, in pairs: one float after the other would round every small one at the size of the largest before it
+template <int G>
+__device__ __forceinline__ float sum_exp(const float (&x)[G], float m) {
+    float e[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) e[j] = exp_neg(x[j] - m);
+#pragma unroll
+    for (int h = G / 2; h > 0; h /= 2)
+#pragma unroll
+        for (int j = 0; j < h; ++j) e[j] += e[j + h];
+    return e[0];
 }
 // for gradients: log2 e as one float (1.3e-8 |t| off, below their own rounding)
 __device__ __forceinline__ float exp_grad(float t) { return __builtin_amdgcn_exp2f(t * 1.44269502162933349609375f); }
@@ -393,14 +405,9 @@ __global__ __launch_bounds__(NT) void logp_rows_kernel(Rows q, PolicyIn p, float
         const float ns = m == -__builtin_huge_valf() ? 0.f : m + spread;      // (nothing but -inf so far: the sum stays 0)
         s = s == 0.0 ? 0.0 : s * (double)exp_neg(ms - ns);
         ms = ns;
-        float a = 0.f;
 #pragma unroll
         for (int i = 0; i < U; ++i)
-            if (k1 + i * NT < n) {      // (whole slots behind the row's end)
-#pragma unroll
-                for (int j = 0; j < E::G; ++j) a += exp_neg(x[i][j] - ms);
-            }
-        s += (double)a;
+            if (k1 + i * NT < n) s += (double)sum_exp(x[i], ms);      // (else: a whole slot behind the row's end)
     }
     double norm = 1.0;
     if constexpr (POLICY) norm = row_norm(p, group_count<NT>(cnt.share(q, p), redi));
@@ -473,18 +480,16 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(Rows q, PolicyIn p, cha
     const double norm = row_norm(p, group_count<NT>(cnt.share(q, p), redi));
     m = group_max<NT>(m, redf);
     only_raw(v);
-    float s = 0.f;
+    double s = 0.0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (NT * i < n) {      // (whole slots behind the row's end)
-            float x[E::G], a = 0.f;
+        if (NT * i < n) {      // (else: a whole slot behind the row's end)
+            float x[E::G];
             E::get(v[i], x);
-#pragma unroll
-            for (int j = 0; j < E::G; ++j) a += exp_neg(x[j] - m);
-            s += a;
+            s += (double)sum_exp(x, m);
         }
     }
-    const double S = group_sum<NT>((double)s, redd);
+    const double S = group_sum<NT>(s, redd);
     only_raw(v);
     if (threadIdx.x == 0) {
         const double lp = ((double)xt - (double)m) - log(S);
