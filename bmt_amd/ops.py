@@ -3609,6 +3609,13 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # BMT_DT_
 _NO_PAD = -(1 << 63)
 # the handle of a device's current stream.  (current_stream() builds a Stream object around it: 2 us of a 10 us call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device      # (there is a tensor on the device: nothing to initialise)
+
+
+def _once_differentiable(backward):
+    """torch's once_differentiable where a backward pass records a graph (create_graph), the plain function where it does not"""
+    recording = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: (recording if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
 def _tuning_device(who: str, *tensors):
@@ -3624,13 +3631,12 @@ def _tuning_device(who: str, *tensors):
             raise ValueError(f"{who}: tensors on {tensors[0].device} and {t.device}")
 
 
-def _run_on(dev: torch.device, what: str, fn, *args):
-    """fn(*args, stream) on the current stream of ``dev``, which need not be the current device"""
-    i = dev.index
-    if torch.cuda.current_device() == i:
+def _run_on(i: int, what: str, fn, *args):
+    """fn(*args, stream) on the current stream of device ``i``, which need not be the current device"""
+    if _current_device() == i:
         rc = fn(*args, _raw_stream(i))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(i):
             rc = fn(*args, _raw_stream(i))
     if rc != 0:
         _lib.check(rc, what)
@@ -3702,7 +3708,7 @@ def _logit_grad(logits, ids, mask, pad_idx, stats_ptr, w_ptr, wb, wt, g, out=Non
         out = _logit_grad_buffer(logits)
     if g is not None and g.dtype != torch.float32:
         g = g.float()
-    _run_on(logits.device, "bmt_logit_grad", lib.bmt_logit_grad, *_row_args(logits, ids, mask, pad_idx), stats_ptr, w_ptr, wb, wt,
+    _run_on(logits.get_device(), "bmt_logit_grad", lib.bmt_logit_grad, *_row_args(logits, ids, mask, pad_idx), stats_ptr, w_ptr, wb, wt,
             None if g is None else g.data_ptr(), int(once), out.data_ptr(), out.stride(0), out.stride(1))
     return out
 
@@ -3722,7 +3728,7 @@ class GenLogitsFn(torch.autograd.Function):
         return handle.logp.view(shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, d):
         (x2,) = ctx.saved_tensors
         W, b = ctx.params
@@ -3742,22 +3748,23 @@ class TokenLogpFn(torch.autograd.Function):
     """log_softmax(logits)[ids], per row; the backward recomputes the softmax from the row's maximum and sum"""
 
     @staticmethod
-    def forward(ctx, logits, ids, mask, pad_idx, recorded):
+    def forward(ctx, logits, rest):
+        ids, mask, pad_idx, recorded = rest
         x = _last_dim_dense(logits)
         B, T, _ = x.shape
         logp = torch.empty(B, T, device=x.device, dtype=torch.float32)
         stats = torch.empty(B, T, 2, device=x.device, dtype=torch.float32) if recorded else None
-        _run_on(x.device, "bmt_logp_rows", lib.bmt_logp_rows, *_row_args(x, ids, mask, pad_idx), logp.data_ptr(), None if stats is None else stats.data_ptr())
+        _run_on(x.get_device(), "bmt_logp_rows", lib.bmt_logp_rows, *_row_args(x, ids, mask, pad_idx), logp.data_ptr(), None if stats is None else stats.data_ptr())
         if recorded:
             ctx.save_for_backward(x, ids, mask, stats)
             ctx.pad_idx = pad_idx
         return logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, d):
         x, ids, mask, stats = ctx.saved_tensors
-        return _logit_grad(x, ids, mask, ctx.pad_idx, stats.data_ptr(), d.data_ptr(), d.stride(0), d.stride(1), None), None, None, None, None
+        return _logit_grad(x, ids, mask, ctx.pad_idx, stats.data_ptr(), d.data_ptr(), d.stride(0), d.stride(1), None), None
 
 
 def token_logp(logits, ids, mask=None, pad_idx: Optional[int] = None):
@@ -3767,7 +3774,7 @@ def token_logp(logits, ids, mask=None, pad_idx: Optional[int] = None):
     _check_rows("token_logp", logits, ids, mask)
     _tuning_device("token_logp", logits, ids, mask)
     logits = _as_logits(logits)
-    return TokenLogpFn.apply(logits, ids, mask, pad_idx, _recorded(logits))
+    return TokenLogpFn.apply(logits, (ids, mask, pad_idx, _recorded(logits)))
 
 
 class PolicyStats:
@@ -3799,7 +3806,8 @@ class PolicyLossFn(torch.autograd.Function):
     a kernel that ends at once if the upstream gradient IS 1 and computes the gradient again, from the logits, if not"""
 
     @staticmethod
-    def forward(ctx, logits, ids, old, adv, ref, mask, pad_idx, lo, hi, beta, reduction, recorded):
+    def forward(ctx, logits, rest):      # (one argument for all that gets no gradient: apply() walks its arguments)
+        ids, old, adv, ref, mask, pad_idx, lo, hi, beta, reduction, recorded = rest
         x = _last_dim_dense(logits)
         B, T, V = x.shape
         dev = x.device
@@ -3813,7 +3821,7 @@ class PolicyLossFn(torch.autograd.Function):
         old, ob, ot = _per_row("policy_loss", "old_logp", old, B, T)
         ref, rb, rt = _per_row("policy_loss", "ref_logp", ref, B, T)
         adv, ab, av = _per_row("policy_loss", "advantages", adv, B, T, per_sequence=True)
-        _run_on(dev, "bmt_policy_loss", lib.bmt_policy_loss, *_row_args(x, ids, mask, pad_idx), None if old is None else old.data_ptr(), ob, ot,
+        _run_on(x.get_device(), "bmt_policy_loss", lib.bmt_policy_loss, *_row_args(x, ids, mask, pad_idx), None if old is None else old.data_ptr(), ob, ot,
                 None if ref is None else ref.data_ptr(), rb, rt, adv.data_ptr(), ab, av, lo, hi, beta, reduction, loss.data_ptr(), info.data_ptr(),
                 info.data_ptr() + 16, ws, n, None if d is None else d.data_ptr(), db, dt)
         if d is not None:
@@ -3824,15 +3832,14 @@ class PolicyLossFn(torch.autograd.Function):
         return loss, info
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, g, _info):
         if g is None:
-            return (None,) * 12
+            return None, None
         x, ids, mask = ctx.saved_tensors
         rows = x.shape[0] * x.shape[1]
         out, ctx.dlogits = ctx.dlogits, None      # (a second backward pass through a kept graph computes its own)
-        d = _logit_grad(x, ids, mask, ctx.pad_idx, ctx.ws + 2048 + 16 * rows, ctx.ws + 2048 + 24 * rows, x.shape[1], 1, g, out)
-        return (d,) + (None,) * 11
+        return _logit_grad(x, ids, mask, ctx.pad_idx, ctx.ws + 2048 + 16 * rows, ctx.ws + 2048 + 24 * rows, x.shape[1], 1, g, out), None
 
 
 def policy_loss(logits, ids, old_logp, advantages, ref_logp=None, mask=None, pad_idx: Optional[int] = None, clip_low: float = 0.2,
@@ -3856,15 +3863,16 @@ def policy_loss(logits, ids, old_logp, advantages, ref_logp=None, mask=None, pad
     if kl_coef != 0 and ref_logp is None:
         raise ValueError(f"policy_loss: a KL term of {kl_coef} needs ref_logp")
     logits = _as_logits(logits)
-    loss, info = PolicyLossFn.apply(logits, ids, old_logp, advantages, ref_logp, mask, pad_idx, float(clip_low), float(clip_high), float(kl_coef),
-                                    _REDUCTIONS[reduction], _recorded(logits))
+    loss, info = PolicyLossFn.apply(logits, (ids, old_logp, advantages, ref_logp, mask, pad_idx, float(clip_low), float(clip_high), float(kl_coef),
+                                             _REDUCTIONS[reduction], _recorded(logits)))
     return loss, PolicyStats(info, ids.shape)
 
 
 class PreferenceLossFn(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, logits, ids, ref, mask, pad_idx, beta, smoothing, mean, recorded):
+    def forward(ctx, logits, rest):
+        ids, ref, mask, pad_idx, beta, smoothing, mean, recorded = rest
         x = _last_dim_dense(logits)
         B, T, V = x.shape
         dev = x.device
@@ -3872,7 +3880,7 @@ class PreferenceLossFn(torch.autograd.Function):
         rewards = torch.empty(B, device=dev, dtype=torch.float32)
         n = lib.bmt_preference_ws_bytes(B, T)
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
-        _run_on(dev, "bmt_preference_loss", lib.bmt_preference_loss, *_row_args(x, ids, mask, pad_idx), ref.data_ptr(), ref.stride(0), beta, smoothing,
+        _run_on(x.get_device(), "bmt_preference_loss", lib.bmt_preference_loss, *_row_args(x, ids, mask, pad_idx), ref.data_ptr(), ref.stride(0), beta, smoothing,
                 int(mean), loss.data_ptr(), rewards.data_ptr(), ws.data_ptr(), n)
         if recorded:
             ctx.save_for_backward(x, ids, mask, ws)
@@ -3882,13 +3890,13 @@ class PreferenceLossFn(torch.autograd.Function):
         return loss, rewards
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, g, _rewards):
         if g is None:
-            return (None,) * 9
+            return None, None
         x, ids, mask, ws = ctx.saved_tensors
         rows = x.shape[0] * x.shape[1]
-        return (_logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr(), ws.data_ptr() + 8 * rows, 1, 0, g),) + (None,) * 8
+        return _logit_grad(x, ids, mask, ctx.pad_idx, ws.data_ptr(), ws.data_ptr() + 8 * rows, 1, 0, g), None
 
 
 def preference_loss(logits, ids, ref_logp, mask=None, pad_idx: Optional[int] = None, beta: float = 0.1, label_smoothing: float = 0.0,
@@ -3907,20 +3915,21 @@ def preference_loss(logits, ids, ref_logp, mask=None, pad_idx: Optional[int] = N
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"preference_loss: label_smoothing {label_smoothing}")
     logits = _as_logits(logits)
-    return PreferenceLossFn.apply(logits, ids, ref_logp, mask, pad_idx, float(beta), float(label_smoothing), bool(mean_logp), _recorded(logits))
+    return PreferenceLossFn.apply(logits, (ids, ref_logp, mask, pad_idx, float(beta), float(label_smoothing), bool(mean_logp), _recorded(logits)))
 
 
 def _embedding_forward(idc, W, scale):
     V, D = W.shape
     out = torch.empty(*idc.shape, D, device=W.device, dtype=W.dtype)
-    _run_on(W.device, "bmt_embedding", lib.bmt_embedding, idc.data_ptr(), W.data_ptr(), W.stride(0) if V > 1 else D, out.data_ptr(), idc.numel(), D, V, _DTYPES[W.dtype], scale)
+    _run_on(W.get_device(), "bmt_embedding", lib.bmt_embedding, idc.data_ptr(), W.data_ptr(), W.stride(0) if V > 1 else D, out.data_ptr(), idc.numel(), D, V, _DTYPES[W.dtype], scale)
     return out
 
 
 class EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, ids, W, scale, pad_idx):
+    def forward(ctx, W, rest):
+        ids, scale, pad_idx = rest
         ctx.save_for_backward(ids)
         ctx.meta = (W.shape, scale, pad_idx)
         ctx.weight = W
@@ -3928,7 +3937,7 @@ class EmbeddingFn(torch.autograd.Function):
         return _embedding_forward(ids, W, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         (V, D), scale, pad_idx = ctx.meta
@@ -3946,11 +3955,11 @@ class EmbeddingFn(torch.autograd.Function):
         dW = torch.empty(V, D, device=dy.device, dtype=dy.dtype) if gW is None else None
         nws = lib.bmt_embedding_bwd_ws_bytes(n, D, V)
         ws = torch.empty(nws, device=dy.device, dtype=torch.uint8)
-        _run_on(dy.device, "bmt_embedding_bwd", lib.bmt_embedding_bwd, ids.data_ptr(), d2.data_ptr(), ld, n, D, V, _DTYPES[dy.dtype], scale,
+        _run_on(dy.get_device(), "bmt_embedding_bwd", lib.bmt_embedding_bwd, ids.data_ptr(), d2.data_ptr(), ld, n, D, V, _DTYPES[dy.dtype], scale,
                 _NO_PAD if pad_idx is None else int(pad_idx), None if dW is None else dW.data_ptr(), None if gW is None else gW.data_ptr(), D, ws.data_ptr(), nws)
         if gW is not None:
             grad_done(ctx.weight)
-        return None, dW, None, None
+        return dW, None
 
 
 def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
@@ -3968,5 +3977,5 @@ def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
         weight = weight.contiguous()
     idc = ids.contiguous()
     if _recorded(weight):
-        return EmbeddingFn.apply(idc, weight, float(scale), pad_idx)
+        return EmbeddingFn.apply(weight, (idc, float(scale), pad_idx))
     return _embedding_forward(idc, weight, float(scale))

@@ -238,7 +238,7 @@ class GradClipper:
         result = torch.empty(2, device=self.device, dtype=torch.float32)
         n = lib.bmt_clip_ws_bytes()
         ws = torch.empty(n, device=self.device, dtype=torch.uint8)      # (of this call: two captured graphs, or two streams, share nothing)
-        _run_on(self.device, "bmt_clip_grads", lib.bmt_clip_grads, self._tiles.data_ptr() if self._n else None, self._n, self._inf, self.max_norm, self.eps,
+        _run_on(self.device.index, "bmt_clip_grads", lib.bmt_clip_grads, self._tiles.data_ptr() if self._n else None, self._n, self._inf, self.max_norm, self.eps,
                 None if scale is None else scale.data_ptr(), int(apply), self._in_place, result.data_ptr(), ws.data_ptr(), n)
         if apply:
             torch.autograd.graph.increment_version(self.out)

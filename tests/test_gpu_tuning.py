@@ -1015,3 +1015,32 @@ def test_embedding_of_more_ids_than_short_chunks_hold(ops):
     want = torch.zeros(V, D, device="cuda", dtype=torch.float64).index_add_(0, ids, dout.double())
     want[PAD] = 0
     assert torch.equal(dW.double(), want)
+
+
+def test_inputs_that_get_no_gradient_may_ask_for_one(ops):
+    g = gen(22)
+    x = torch.randn(2, 3, 20, device="cuda", generator=g)
+    ids = torch.randint(0, 20, (2, 3), device="cuda", generator=g)
+    old, adv, ref = (torch.randn(2, 3, device="cuda", generator=g).requires_grad_(True) for _ in range(3))
+    loss, _ = ops.policy_loss(x, ids, old, adv, ref, kl_coef=0.1)
+    assert not loss.requires_grad
+    pair, _ = ops.preference_loss(x, ids, torch.zeros(2, device="cuda", requires_grad=True))
+    assert not pair.requires_grad
+    x.requires_grad_(True)
+    again, _ = ops.policy_loss(x, ids, old, adv, ref, kl_coef=0.1)
+    dx, dold = torch.autograd.grad(again, (x, old), allow_unused=True)
+    assert torch.equal(again, loss) and dold is None and bool((dx != 0).any())
+
+
+def test_a_gradient_of_a_gradient_is_refused(ops):
+    x = torch.randn(2, 3, 20, device="cuda").requires_grad_(True)
+    W = torch.randn(20, 4, device="cuda").requires_grad_(True)
+    ids = torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    row = torch.ones(2, 3, device="cuda")
+    for leaf, call in ((x, lambda: ops.policy_loss(x, ids, row, row)[0]), (x, lambda: ops.preference_loss(x, ids, torch.zeros(2, device="cuda"))[0]),
+                       (x, lambda: ops.token_logp(x, ids).sum()), (W, lambda: ops.embedding(ids, W).sum())):
+        (d,) = torch.autograd.grad(call(), leaf)
+        (same,) = torch.autograd.grad(call(), leaf, create_graph=True)
+        assert torch.equal(d, same)
+        with pytest.raises(RuntimeError):
+            same.sum().backward()
