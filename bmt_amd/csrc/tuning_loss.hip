@@ -11,7 +11,7 @@
 // Rows that do not count (mask 0, or the padding id) are not read; their gradient rows are written as zeros.
 // Measured: policy loss with its gradient, all rows counting, 8192 x 32000 bf16 202 us (5.2 TB/s of logits read + gradients written; a plain copy
 // reaches 5.95), 65536 x 1000 bf16 78 us; preference loss 16 x 1024 x 32000 bf16, a third of the rows masked: 121 us for the log-probabilities (5.7 TB/s
-// of the rows read), 292 us for the gradient (5.9 TB/s).
+// of the rows read), 291 us for the gradient (5.9 TB/s).
 #include "common.h"
 
 namespace {
