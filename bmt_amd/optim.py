@@ -191,6 +191,8 @@ class GradClipper:
         for g, o in zip(self.grads, self.out):
             if g.shape != o.shape or any(a != 1 and g.numel() > 0 and x != y for a, x, y in zip(g.shape, g.stride(), o.stride())):
                 raise ValueError(f"GradClipper: a gradient of shape {tuple(g.shape)} and strides {g.stride()} with an output of {tuple(o.shape)} and {o.stride()}")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("GradClipper: make the plan before the capture (its table is copied from the host); calls of it are captured")
         self.device = self.grads[0].device
         self._ptrs = [t.data_ptr() for t in self.grads], [t.data_ptr() for t in self.out]
         self._in_place = int(all(g.dtype == o.dtype for g, o in zip(self.grads, self.out)) and self._ptrs[0] == self._ptrs[1])

@@ -1044,3 +1044,19 @@ def test_a_gradient_of_a_gradient_is_refused(ops):
         assert torch.equal(d, same)
         with pytest.raises(RuntimeError):
             same.sum().backward()
+
+
+def test_a_clipping_plan_is_not_made_inside_a_capture():
+    from bmt_amd.optim import GradClipper
+    t = torch.ones(100, device="cuda")
+    plan = GradClipper([t], 1.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            GradClipper([t], 1.0)
+        norm = plan()
+    for _ in range(2):
+        t.fill_(1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert abs(float(norm) - 10.0) < 1e-5 and abs(float(t.norm()) - 1.0) < 1e-5
