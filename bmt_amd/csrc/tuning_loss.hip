@@ -265,10 +265,10 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
     return s;
 }
 
-// e^d - 1 - d.  Policies that are compared lie close together: up to 1/2 by its series (15 terms: below 1e-16 of it), without cancellation and without
-// the library's exponential, which is long for the one thread that works while the workgroup waits
+// e^d - 1 - d for |d| <= 1/2.  Policies that are compared lie close together: a series there (15 terms: below 1e-16 of it), without cancellation and
+// without the library's exponential, which is long for the one thread that works while the workgroup waits
+constexpr double NEAR = 0.5;
 __device__ __forceinline__ double exp_rest(double d) {
-    if (!(fabs(d) <= 0.5)) return exp(d) - 1.0 - d;      // (NaN goes this way)
     double s = 1.0;
 #pragma unroll
     for (int k = 15; k > 2; --k) s = fma(s * d, 1.0 / k, 1.0);
@@ -284,16 +284,23 @@ __device__ __forceinline__ double row_norm(const PolicyIn& p, int counted) {
 // KL term is second order in them.  Returns w_r
 __device__ __forceinline__ float policy_row(const PolicyIn& p, const RowIn& in, double norm, double lp, Terms* terms) {
     const double A = in.adv, dold = lp - (p.old ? (double)in.old : lp);      // (lp - lp: NaN stays NaN)
-    const double rho = fabs(dold) <= 0.5 ? 1.0 + dold + exp_rest(dold) : exp(dold);      // (a token of probability 0 now: 0)
+    const double rho = fabs(dold) <= NEAR ? 1.0 + dold + exp_rest(dold) : exp(dold);      // (a token of probability 0 now: 0)
     const double u = rho * A, c = fmin(fmax(rho, 1.0 - (double)p.lo), 1.0 + (double)p.hi) * A;
     const bool clipped = u > c;
     double loss = clipped ? -c : -u, w = clipped ? 0.0 : -u, kl = 0.0;
     if (p.ref) {
         const double d = (double)in.ref - lp;
-        kl = exp_rest(d);
+        double em;      // e^d - 1: -1 for a token that the reference rules out (d = -inf, or a type's lowest value), whose KL term is beyond any bound
+        if (fabs(d) <= NEAR) {
+            kl = exp_rest(d);
+            em = d + kl;
+        } else {        // (NaN goes this way)
+            em = exp(d) - 1.0;
+            kl = em - d;
+        }
         if (p.beta != 0.f) {      // (a term that is only watched may be infinite: 0 * inf)
             loss += (double)p.beta * kl;
-            w -= (double)p.beta * (kl + d);
+            w -= (double)p.beta * em;
         }
     }
     *terms = Terms{loss * norm, (float)kl, clipped ? 3 : 1};
