@@ -2495,9 +2495,12 @@ class GeneratorFn(torch.autograd.Function):
         x2, W, logp = ctx.saved_tensors
         V = W.shape[0]
         d2 = _f32c(dlogp).view(-1, V)
-        dlogits = torch.empty_like(d2)
-        _lib.check(lib.bmt_log_softmax_bwd(_p(logp), logp.stride(0), _p(d2), d2.stride(0), _p(dlogits), dlogits.stride(0),
-                                           d2.shape[0], V, _st()), "bmt_log_softmax_bwd")
+        if _rows_sum_to_zero(dlogp):          # (dlogits = d - softmax * its row's sum)
+            dlogits = d2
+        else:
+            dlogits = torch.empty_like(d2)
+            _lib.check(lib.bmt_log_softmax_bwd(_p(logp), logp.stride(0), _p(d2), d2.stride(0), _p(dlogits), dlogits.stride(0),
+                                               d2.shape[0], V, _st()), "bmt_log_softmax_bwd")
         Wp, bp = ctx.params
         dx, dW, db = lin_bwd(dlogits, Wp, bp, x2, need_dx=ctx.needs_input_grad[0])
         if dx is not None:
@@ -3714,34 +3717,33 @@ def _logit_grad(logits, ids, mask, pad_idx, stats_ptr, w_ptr, wb, wt, g, out=Non
 
 
 class GenLogitsFn(torch.autograd.Function):
-    """A Generator's log-probabilities as the logits of a loss from logits, as a node of its own over the generator's input and parameters: such a
-    loss takes log-softmax itself (which leaves log-probabilities as they are), its gradient sums to zero over a row, and the way back through the
-    generator's log-softmax (GeneratorFn: three passes over the (B*Tc, V) tensor) would return the same values"""
+    """A Generator's log-probabilities as the logits of a loss from logits: the same values, behind a node that says of the gradient that its rows
+    sum to zero (such a loss takes log-softmax itself, which leaves log-probabilities as they are, and so its gradient does).  GeneratorFn goes back
+    through its products directly then: the way through its own log-softmax, three passes over the (B*Tc, V) tensor, would return the same values.
+    The gradient passes the Generator's output itself: its hooks see it, and GeneratorFn's checks of what it saved hold"""
 
     @staticmethod
-    def forward(ctx, x, W, b, handle, shape):
-        note_use(W, b)
-        xc = _f32c(x)
-        ctx.save_for_backward(xc.view(-1, xc.shape[-1]))
-        ctx.params, ctx.xshape = (W, b), x.shape
-        _settle_later(handle)
-        return handle.logp.view(shape)
+    def forward(ctx, pred):
+        return pred.detach()
 
     @staticmethod
-    @_once_differentiable
     def backward(ctx, d):
-        (x2,) = ctx.saved_tensors
-        W, b = ctx.params
-        dx, dW, db = lin_bwd(_f32c(d).view(-1, W.shape[0]), W, b, x2, need_dx=ctx.needs_input_grad[0])
-        return None if dx is None else dx.view(ctx.xshape), dW, db, None, None
+        d._bmt_zero_sum = d._version
+        return d
+
+
+def _rows_sum_to_zero(d) -> bool:
+    """whether ``d`` is a gradient that GenLogitsFn handed on, and nothing was added to it or written into it since (the engine adds the gradients
+    of several consumers to a new tensor, or in place: another version)"""
+    return getattr(d, "_bmt_zero_sum", None) == d._version
 
 
 def _as_logits(pred):
     """pred, or -- a Generator's untouched output in a pass that records a graph -- its values behind GenLogitsFn"""
     h = getattr(pred, "_bmt_gen", None)
-    if not FUSE_GEN_LOSS or h is None or h.logp is None or not _recorded(pred) or generator_handle(pred) is None:
+    if not FUSE_GEN_LOSS or h is None or h.version != pred._version or not _recorded(pred):
         return pred
-    return GenLogitsFn.apply(h.x, h.W, h.b, h, pred.shape)
+    return GenLogitsFn.apply(pred)
 
 
 class TokenLogpFn(torch.autograd.Function):

@@ -56,3 +56,138 @@ def test_gradient_of_the_kl_term_for_any_reference(ops, dtype, V):
     rest, _ = ops.policy_loss(x[3:], ids[3:], old[3:], adv[3:], ref[3:], kl_coef=beta, reduction="sum")
     total = (-adv.double()[3:, None] * torch.exp(lp - old.double())[3:] + beta * (torch.expm1(d) - d)[3:]).sum()
     within(rest, total, 2 * U * abs(float(total)), "loss")          # (1e16 of it: the loss's own rounding, and beta is exact)
+
+
+# ----------------------------------------------------------------------------- losses on a Generator's own output
+def behind_a_generator(V=203, D=48, B=4, T=7):
+    from bmt_amd.model.generators import Generator
+    torch.manual_seed(0)
+    generator, g = Generator(D, V).cuda(), gen(12)
+    x = torch.randn(B, T, D, device="cuda", generator=g).requires_grad_(True)
+    ids = torch.randint(2, V, (B, T), device="cuda", generator=g)
+    old, adv = torch.full((B, T), -5.3, device="cuda"), torch.randn(B, device="cuda", generator=g)
+    seq = torch.zeros(B, device="cuda")
+    from bmt_amd import ops
+    losses = {"policy": lambda p: ops.policy_loss(p, ids, old, adv)[0], "policy_times_3": lambda p: ops.policy_loss(p, ids, old, adv)[0] * 3.0,
+              "logp": lambda p: ops.token_logp(p, ids).square().mean(), "preference": lambda p: ops.preference_loss(p, ids, seq)[0]}
+    return generator, x, losses
+
+
+LOSSES = ["policy", "policy_times_3", "logp", "preference"]
+
+
+@pytest.mark.parametrize("name", LOSSES)
+def test_a_generator_s_output_sees_its_gradient(ops, monkeypatch, name):
+    """hooks, retain_grad and torch.autograd.grad on the output itself get what the loss gives logits that are leaves, and the way behind the output
+    runs without the log-softmax's backward"""
+    generator, x, losses = behind_a_generator()
+    calls = []
+    monkeypatch.setattr(ops.lib, "bmt_log_softmax_bwd", lambda *a, f=ops.lib.bmt_log_softmax_bwd: (calls.append(1), f(*a))[1])
+    pred = generator(x)
+    leaf = pred.detach().clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(losses[name](leaf), leaf)
+    (got,) = torch.autograd.grad(losses[name](pred), pred, retain_graph=True)
+    assert torch.equal(got, want)
+    seen = []
+    pred.retain_grad()
+    pred.register_hook(lambda g: seen.append(g.clone()))
+    losses[name](pred).backward()
+    assert len(seen) == 1 and torch.equal(seen[0], want) and torch.equal(pred.grad, want)
+    assert not calls
+    (losses[name](generator(x)) + losses[name](generator(x)) * 0.0).backward()
+    assert not calls
+    pred = generator(x)
+    (losses[name](pred) + pred.mean()).backward()          # another consumer: the sum of the gradients goes the whole way
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize("name", LOSSES)
+def test_the_way_past_a_generator_s_log_softmax(ops, monkeypatch, name):
+    """the same gradients as through it: fp32 roundings of the logits' gradient, after which every operand is a bf16 plane, where one of them moves a
+    value by at most a step, 2^-7 of it"""
+    generator, x, losses = behind_a_generator()
+    leaves, got = [x, generator.linear.weight, generator.linear.bias], {}
+    for fused in (True, False):
+        monkeypatch.setattr(ops, "FUSE_GEN_LOSS", fused)
+        got[fused] = torch.autograd.grad(losses[name](generator(x)), leaves)
+    for a, b in zip(got[True], got[False]):
+        assert float((a - b).double().norm()) <= 2.0 ** -7 * float(b.double().norm())
+
+
+@pytest.mark.parametrize("what", ["weight", "output"])
+def test_a_generator_written_to_before_the_backward_pass_is_noticed(ops, what):
+    generator, x, losses = behind_a_generator()
+    for name in LOSSES:
+        pred = generator(x)
+        loss = losses[name](pred)
+        with torch.no_grad():
+            (generator.linear.weight if what == "weight" else pred).mul_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+class Watched(torch.autograd.Function):
+    """a node in front of the generator that holds an object: alive as long as the pass is"""
+
+    @staticmethod
+    def forward(ctx, x, held):
+        ctx.held = held
+        return x * 1.0
+
+    @staticmethod
+    def backward(ctx, d):
+        return d, None
+
+
+class Held:
+    pass
+
+
+@pytest.mark.parametrize("backward", [True, False])
+@pytest.mark.parametrize("name", LOSSES)
+def test_a_pass_ends_with_its_loss(ops, name, backward):
+    """once loss and output are dropped nothing of a pass lives on: neither the log-probabilities nor the graph in front of the generator"""
+    import gc
+    import weakref
+    generator, x, losses = behind_a_generator()
+    ops.context().gen_handles.clear()
+    sizes, held = [], []
+    for _ in range(4):
+        h = Held()
+        held.append(weakref.ref(h))
+        pred = generator(Watched.apply(x, h))
+        loss = losses[name](pred)
+        if backward:
+            loss.backward()
+        del pred, loss, h
+        gc.collect()
+        sizes.append(torch.cuda.memory_allocated())
+        assert held[-1]() is None
+    assert sizes[1] == sizes[2] == sizes[3] and not ops.context().gen_handles
+
+
+@pytest.mark.parametrize("name", LOSSES)
+def test_a_generator_with_static_gradient_buffers(ops, name):
+    """GradientReducer, a loss on the generator's output, GradClipper: the buffers hold the gradients, and every use of a parameter that the forward
+    pass counted is settled by the backward pass alone, step after step"""
+    from bmt_amd.optim import GradClipper
+    from bmt_amd.parallel import GradientReducer
+    generator, x, losses = behind_a_generator()
+    params = [generator.linear.weight, generator.linear.bias]
+    want = torch.autograd.grad(losses[name](generator(x)), params)
+    reducer = GradientReducer(params)
+    try:
+        clipper = GradClipper([p.grad for p in params], max_norm=1e9)
+        for _ in range(3):
+            reducer.zero_grad()
+            losses[name](generator(x)).backward()
+            assert all(p._bmt_uses == 0 for p in params) and not ops.context().gen_handles
+            reducer.finish()
+            norm = clipper()
+            for p, w in zip(params, want):
+                # (sums over 28 rows of the same operands, in another order: 28 u of their absolute sum, which stays below 28 times the largest)
+                assert float((p.grad - w).abs().max()) <= 28 * 28 * U * float(w.abs().max())
+            total = sum(float(p.grad.double().square().sum()) for p in params) ** 0.5
+            assert abs(float(norm) - total) <= 2 * U * total
+    finally:
+        reducer.remove()
