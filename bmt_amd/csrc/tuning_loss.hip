@@ -598,8 +598,9 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
         const Row<DT> row(xr, q.V);
         const int n = row.granules();
         const float2 st = stats[r];
-        const float wr = w[b * wb + t * wt] * gs, m = st.x, c = -wr * st.y;
-        const int kt = (int)((row.phase + id) / E::G), jt = (int)((row.phase + id) % E::G);
+        const bool known = id >= 0 && id < q.V;      // (an id outside the vocabulary has no log-probability, and its row no gradient: NaN)
+        const float wr = known ? w[b * wb + t * wt] * gs : __builtin_nanf(""), m = st.x, c = -wr * st.y;
+        const int at = row.phase + (known ? (int)id : 0), kt = at / E::G, jt = at % E::G;
         for (int k = threadIdx.x; k < n; k += NT) {
             float x[E::G];
             E::get(row.template load<true>(k), x);

@@ -191,3 +191,36 @@ def test_a_generator_with_static_gradient_buffers(ops, name):
             assert abs(float(norm) - total) <= 2 * U * total
     finally:
         reducer.remove()
+
+
+# ----------------------------------------------------------------------------- ids outside the vocabulary
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("V", [7, 1000, 140001])
+def test_ids_outside_the_vocabulary_give_nan_rows(ops, dtype, V):
+    """value and gradient of such a row are NaN throughout, whichever loss asks and however far outside the id is; other rows are as without it"""
+    g = gen(V)
+    outside = [-1, V, V + 13, -(1 << 40), (1 << 35) + 3, (1 << 62)]
+    B, T = len(outside) + 2, 2
+    x = torch.randn(B, T, V, device="cuda", generator=g).to(dtype).requires_grad_(True)
+    good = torch.randint(0, V, (B, T), device="cuda", generator=g)
+    ids = good.clone()
+    ids[:len(outside), 0] = torch.tensor(outside, device="cuda")
+    bad = ids != good
+    up = torch.randn(B, T, device="cuda", generator=g)
+    lp, lp_good = ops.token_logp(x, ids), ops.token_logp(x, good)
+    assert bool(torch.isnan(lp[bad]).all()) and torch.equal(lp[~bad], lp_good[~bad])
+    (dx,), (want,) = torch.autograd.grad(lp, x, up), torch.autograd.grad(lp_good, x, up)
+    assert bool(torch.isnan(dx[bad]).all()) and torch.equal(dx[~bad], want[~bad])
+    loss, _ = ops.policy_loss(x, ids, None, up, reduction="sum")
+    (dx,) = torch.autograd.grad(loss, x, retain_graph=True)
+    (dx2,) = torch.autograd.grad(loss * 2.0, x)
+    assert torch.isnan(loss) and all(bool(torch.isnan(d[bad]).all()) and bool(torch.isfinite(d[~bad]).all()) for d in (dx, dx2))
+    loss, rewards = ops.preference_loss(x, ids, torch.zeros(B, device="cuda"))
+    (dx,) = torch.autograd.grad(loss, x)
+    hit = bad.any(1)
+    pair = hit[:B // 2] | hit[B // 2:]
+    assert torch.isnan(loss) and torch.equal(torch.isnan(rewards), hit)
+    assert torch.equal(torch.isnan(dx).all(2).all(1), pair.repeat(2)) and bool(torch.isfinite(dx[~pair.repeat(2)]).all())
+    masked = ids.clone()
+    mask = ~bad
+    assert bool(torch.isfinite(torch.autograd.grad(ops.policy_loss(x, masked, None, up, mask=mask)[0], x)[0]).all())
