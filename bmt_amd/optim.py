@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _p, _run_on, _st, lib
+from .ops import _DTYPES, _p, _raw_stream, _run_on, _st, lib
 
 
 class _PtrTable:
@@ -199,6 +199,7 @@ class GradClipper:
         self._refuse_shared_memory()
         self.coef = None
         self._tiles, self._n = self._table()
+        self._stream = _raw_stream(self.device.index)      # whose memory the table is
 
     def _refuse_shared_memory(self):
         ranges = []
@@ -235,8 +236,11 @@ class GradClipper:
             raise RuntimeError("GradClipper: a tensor's memory has moved since the plan was made: make a new one")
         if scale is not None and (scale.numel() != 1 or scale.dtype != torch.float32 or scale.device != self.device):
             raise ValueError(f"GradClipper: scale is one float32 value on {self.device}")
-        if torch.cuda.is_current_stream_capturing() and not any(t is self._tiles for t in _captured_tables):
-            _captured_tables.append(self._tiles)
+        if torch.cuda.is_current_stream_capturing():
+            if not any(t is self._tiles for t in _captured_tables):
+                _captured_tables.append(self._tiles)
+        elif _raw_stream(self.device.index) != self._stream:      # (a plan dropped behind this call: its table outlives what this stream still runs)
+            self._tiles.record_stream(torch.cuda.current_stream(self.device))
         result = torch.empty(2, device=self.device, dtype=torch.float32)
         n = lib.bmt_clip_ws_bytes()
         ws = torch.empty(n, device=self.device, dtype=torch.uint8)      # (of this call: two captured graphs, or two streams, share nothing)

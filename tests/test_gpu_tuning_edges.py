@@ -224,3 +224,31 @@ def test_ids_outside_the_vocabulary_give_nan_rows(ops, dtype, V):
     masked = ids.clone()
     mask = ~bad
     assert bool(torch.isfinite(torch.autograd.grad(ops.policy_loss(x, masked, None, up, mask=mask)[0], x)[0]).all())
+
+
+# ----------------------------------------------------------------------------- clipping plans
+def test_a_clipping_plan_dropped_behind_a_call_on_another_stream(ops):
+    """its tile table belongs to the stream it was made on; while a call on another stream may still read it, that memory goes to nobody else"""
+    from bmt_amd.optim import GradClipper
+    work = torch.randn(4096, 4096, device="cuda")
+    grads = [torch.full((100003,), 0.5, device="cuda"), torch.full((33,), 0.25, device="cuda")]
+    plan = GradClipper(grads, max_norm=1.0)
+    table = (plan._tiles.data_ptr(), plan._tiles.numel())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(50):          # (tens of milliseconds in front of the call)
+            work = work @ work
+            work = work / work.norm()
+        norm = plan()
+        behind = side.record_event()
+    del plan
+    taken = [torch.empty(table[1], dtype=torch.uint8, device="cuda") for _ in range(64)]
+    where = [t.data_ptr() for t in taken]
+    still_running = not behind.query()
+    side.synchronize()
+    assert still_running and table[0] not in where
+    want = (100003 * 0.25 + 33 * 0.0625) ** 0.5
+    assert abs(float(norm) - want) <= 2 * U * want
+    for t, v in zip(grads, (0.5, 0.25)):
+        assert float((t - v / (want + 1e-6)).abs().max()) <= 4 * U * v / want
