@@ -172,14 +172,14 @@ class GradClipper:
     def __init__(self, grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None, norm_type: float = 2.0, eps: float = 1e-6):
         self.grads = list(grads)
         self.out = self.grads if out is None else list(out)
-        self.max_norm, self.eps = float(max_norm), float(eps)
+        self.max_norm, self.eps = max_norm, float(eps)
         if not self.grads:
             raise ValueError("GradClipper: no gradients")
         if norm_type not in (2, float("inf")):
             raise ValueError(f"GradClipper: norm_type {norm_type} (2 or inf)")
         self._inf = int(norm_type != 2)
-        if not (self.max_norm >= 0.0 and self.eps >= 0.0):
-            raise ValueError(f"GradClipper: max_norm {max_norm}, eps {eps}")
+        if not self.eps >= 0.0:
+            raise ValueError(f"GradClipper: eps {eps}")
         if len(self.out) != len(self.grads):
             raise ValueError(f"GradClipper: {len(self.out)} output tensors for {len(self.grads)} gradients")
         for t in self.grads + ([] if out is None else self.out):
@@ -200,6 +200,17 @@ class GradClipper:
         self.coef = None
         self._tiles, self._n = self._table()
         self._stream = _raw_stream(self.device.index)      # whose memory the table is
+
+    @property
+    def max_norm(self) -> float:
+        """the bound: an argument of every call, so it may be set anew between calls"""
+        return self._max_norm
+
+    @max_norm.setter
+    def max_norm(self, value: float):
+        if not float(value) >= 0.0:
+            raise ValueError(f"GradClipper: max_norm {value}")
+        self._max_norm = float(value)
 
     def _refuse_shared_memory(self):
         ranges = []
@@ -244,7 +255,7 @@ class GradClipper:
         result = torch.empty(2, device=self.device, dtype=torch.float32)
         n = lib.bmt_clip_ws_bytes()
         ws = torch.empty(n, device=self.device, dtype=torch.uint8)      # (of this call: two captured graphs, or two streams, share nothing)
-        _run_on(self.device.index, "bmt_clip_grads", lib.bmt_clip_grads, self._tiles.data_ptr() if self._n else None, self._n, self._inf, self.max_norm, self.eps,
+        _run_on(self.device.index, "bmt_clip_grads", lib.bmt_clip_grads, self._tiles.data_ptr() if self._n else None, self._n, self._inf, self._max_norm, self.eps,
                 None if scale is None else scale.data_ptr(), int(apply), self._in_place, result.data_ptr(), ws.data_ptr(), n)
         if apply:
             torch.autograd.graph.increment_version(self.out)

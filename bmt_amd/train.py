@@ -183,8 +183,9 @@ class CaptioningTrainStep:
         if self.cfg.grad_clip is not None and self._fused_scale and self.reducer is not None:
             # static gradient buffers: normaliser and clipping in two launches over the arena (what the two passes below leave in p.grad,
             # from one factor instead of two), the same sums on every run, and nothing in it that a hipGraph cannot replay
-            if self._clipper is None or self._clipper.max_norm != float(self.cfg.grad_clip):
+            if self._clipper is None:
                 self._clipper = GradClipper([self.reducer._arena], self.cfg.grad_clip)
+            self._clipper.max_norm = float(self.cfg.grad_clip)      # (an argument of the call: another bound needs no other plan, also inside a capture)
             self._clipper(scale=self.grad_scale)
             self.optimizer.grad_scale = None
             try:

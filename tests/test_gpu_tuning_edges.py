@@ -252,3 +252,28 @@ def test_a_clipping_plan_dropped_behind_a_call_on_another_stream(ops):
     assert abs(float(norm) - want) <= 2 * U * want
     for t, v in zip(grads, (0.5, 0.25)):
         assert float((t - v / (want + 1e-6)).abs().max()) <= 4 * U * v / want
+
+
+def test_another_clipping_bound_in_front_of_a_capture_without_warm_up(ops):
+    """cfg.grad_clip may change between eager steps and a capture that runs none of its own"""
+    from tests.test_gpu_tuning import caption_step
+    step, fs, caps = caption_step(1e6)
+    for _ in range(2):
+        step(fs, caps)
+    step.cfg.grad_clip = 0.05
+    step.capture(fs, caps, warmup=0)
+    for _ in range(3):
+        step.replay(fs, caps)
+        torch.cuda.synchronize()
+        total = sum(float(p.grad.double().square().sum()) for p in step.params) ** 0.5
+        # (clipped: the norm is at least 0.05, so eps = 1e-6 takes at most 2e-5 of the total; the factor and every product are rounded)
+        assert abs(total - 0.05) <= 0.05 * (2e-5 + 8 * U)
+        float(sum(p.sum() for p in step.params))          # (the program's own work between the replays)
+    step.uncapture()
+    step.cfg.grad_clip = 0.025
+    step(fs, caps)
+    total = sum(float(p.grad.double().square().sum()) for p in step.params) ** 0.5
+    assert abs(total - 0.025) <= 0.025 * (4e-5 + 8 * U)
+    for bound in (-1.0, float("nan")):
+        with pytest.raises(ValueError):
+            step._clipper.max_norm = bound
