@@ -1,7 +1,9 @@
 // Scaled embedding lookup and its gradient by sorted tokens.
 //   out[n] = scale W[id_n]                              dW[v] = scale sum_{n : id_n = v} dout[n]
 // Bound: HBM -- the lookup reads N rows and writes N rows, the gradient reads N rows and writes V rows, one or two operations per element.
-// The gradient sums in fp32 over the positions of a token in ascending order, rounded once: no atomics, the same bits on every run.  Three launches:
+// The gradient of a token is the sum over its positions in ascending order, rounded once: in fp32 up to 32 positions (up to N of them where N <= 2048),
+// in fp32 per 32 sorted positions and in 64 bits over those beyond.  The same bits on every run: no atomics among the summands; a static gradient buffer
+// takes each finished row by one atomic addition per element, as other uses of the table may add to it from other streams.  Three launches:
 //   order  workgroup g of G owns the tokens v = g (mod G) -- frequent tokens are neighbours in most vocabularies, and contiguous ranges would give
 //          one workgroup half of a text --, reads ALL ids (they come from L2: 8 bytes against a row of hundreds) and places the positions of its
 //          tokens, in order, behind the count of the tokens of lower owners: no second pass over a global histogram.  Many ids are split by owner
@@ -350,25 +352,25 @@ __device__ __forceinline__ void add_rows(const char* dout, int64_t ld, const int
 
 // dW[v] = scale acc, or (into != NULL: a static fp32 gradient buffer) into[v] += scale acc -- one addition per row and call, in the memory's own
 // add: another use of the table may be adding its gradient from another stream
-template <int DT, int G>
-__device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, int v, int c, int D, float scale, const float (&acc)[G]) {
+template <int DT, int G, typename A>
+__device__ __forceinline__ void finish_row(char* dW, float* into, int64_t ldw, int v, int c, int D, float scale, const A (&acc)[G]) {
     float x[G];
     const int at = cols_at<G>(c, D);
     if (into) {
         float* p = into + (int64_t)v * ldw + at;
 #pragma unroll
         for (int j = 0; j < G; ++j)
-            if (at + j >= c) unsafeAtomicAdd(p + j, scale * acc[j]);      // (each column once)
+            if (at + j >= c) unsafeAtomicAdd(p + j, (float)((A)scale * acc[j]));      // (each column once)
         return;
     }
 #pragma unroll
-    for (int j = 0; j < G; ++j) x[j] = scale * acc[j];
+    for (int j = 0; j < G; ++j) x[j] = (float)((A)scale * acc[j]);
     Cols<DT, G>::store(dW + ((int64_t)v * ldw + at) * elem_size<DT>(), x);
 }
 
 // the four waves' sums into wave 0, in order
-template <int G, int NB>
-__device__ __forceinline__ void join_waves(float (&acc)[NB][G], float (&red)[3][NB][64 * G], int wave, int lane) {
+template <int G, int NB, typename A>
+__device__ __forceinline__ void join_waves(A (&acc)[NB][G], A (&red)[3][NB][64 * G], int wave, int lane) {
     __syncthreads();
     if (wave > 0)
 #pragma unroll
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
             const int q0 = max(p0, a), q1 = min(p1, b), each = (q1 - q0 + 3) / 4;
             float acc[NB][G] = {};
             add_rows<DT, G, NB>(dout, ld, order, min(q1, q0 + wave * each), min(q1, q0 + (wave + 1) * each), c, D, acc);
-            join_waves<G, NB>(acc, red, wave, lane);
+            join_waves<G, NB, float>(acc, red, wave, lane);
             if (wave == 0)
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
         add_rows<DT, G, NB>(dout, ld, order, a, b, c, D, acc);
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            if (c + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, v, c + j * 64 * G, D, scale, acc[j]);
+            if (c + j * 64 * G < D) finish_row<DT, G, float>(dW, into, ldw, v, c + j * 64 * G, D, scale, acc[j]);
     }
     if (chunks) return;
     // no partial sums: the four waves share each frequent token that one of them met
@@ -442,19 +444,20 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const char* __restrict__
         const int mc = (m.w * NB * 64 + lane) * G, each = (m.y - m.x + 3) / 4;
         float acc[NB][G] = {};
         add_rows<DT, G, NB>(dout, ld, order, min(m.y, m.x + wave * each), min(m.y, m.x + (wave + 1) * each), mc, D, acc);
-        join_waves<G, NB>(acc, red, wave, lane);
+        join_waves<G, NB, float>(acc, red, wave, lane);
         if (wave == 0)
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-                if (mc + j * 64 * G < D) finish_row<DT, G>(dW, into, ldw, m.z, mc + j * 64 * G, D, scale, acc[j]);
+                if (mc + j * 64 * G < D) finish_row<DT, G, float>(dW, into, ldw, m.z, mc + j * 64 * G, D, scale, acc[j]);
     }
 }
 
-// a workgroup per (chunk, block of columns): the frequent token whose run starts in the chunk, if there is one -- it holds the chunk's last position
+// a workgroup per (chunk, block of columns): the frequent token whose run starts in the chunk, if there is one -- it holds the chunk's last position.
+// Its partial sums, as many as its positions / EMB_LONG, are added in 64 bits: in 32 the error would grow with how frequent the token is
 template <int DT, int G>
 __global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__ offsets, const int* __restrict__ slot, const float* __restrict__ part, int64_t ldp,
                                                           char* __restrict__ dW, float* __restrict__ into, int64_t ldw, int D, Owners ow, int slots, float scale, int ncb) {
-    __shared__ float red[3][1][64 * G];
+    __shared__ double red[3][1][64 * G];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int k = blockIdx.x / ncb, c = ((int)(blockIdx.x % ncb) * 64 + lane) * G;
     const bool in = c < D;
@@ -464,17 +467,17 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const int* __restrict__
     if (a < p0 || b - a <= EMB_LONG) return;
     const int k1 = (b - 1) / EMB_LONG, n = k1 - k + 1, each = (n + 3) / 4;      // partial sums: slot 0 or 1 of chunk k, slot 0 of the following ones
     const int i0 = min(n, wave * each), i1 = min(n, (wave + 1) * each);
-    float acc[1][G] = {};
+    double acc[1][G] = {};
     if (in) {
 #pragma unroll 4
         for (int i = i0; i < i1; ++i) {
             const float* o = part + (int64_t)(2 * (k + i) + (i == 0 && a > p0 ? 1 : 0)) * ldp + cols_at<G>(c, D);
 #pragma unroll
-            for (int j = 0; j < G; ++j) acc[0][j] += o[j];
+            for (int j = 0; j < G; ++j) acc[0][j] += (double)o[j];
         }
     }
-    join_waves<G, 1>(acc, red, wave, lane);
-    if (wave == 0 && in) finish_row<DT, G>(dW, into, ldw, ow.token(u), c, D, scale, acc[0]);
+    join_waves<G, 1, double>(acc, red, wave, lane);
+    if (wave == 0 && in) finish_row<DT, G, double>(dW, into, ldw, ow.token(u), c, D, scale, acc[0]);
 }
 
 constexpr int64_t MAX_GRID = 0xffffffff / 256;      // workgroups of 256 threads

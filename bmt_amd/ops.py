@@ -3966,8 +3966,8 @@ class EmbeddingFn(torch.autograd.Function):
 
 def embedding(ids, weight, scale: float = 1.0, pad_idx: Optional[int] = None):
     """scale * weight[ids] (ids int64 of any shape; weight (V, D) fp32, bf16 or fp16; ids outside the table are clamped, as EmbedFn does).  The
-    gradient of ``weight`` is added in fp32 over a token's positions in ascending order and rounded once -- the same bits on every run, whichever
-    tokens repeat --; ``pad_idx`` and ids that are clamped to it get none.  A parameter with a static gradient buffer (GradientReducer) has it added there directly."""
+    gradient of ``weight`` is added over a token's positions in ascending order (fp32; 64 bits over the sums of 32 of a frequent token) and rounded
+    once -- the same bits on every run, whichever tokens repeat --; ``pad_idx`` and ids that are clamped to it get none.  A parameter with a static gradient buffer (GradientReducer) has it added there directly."""
     _tuning_device("embedding", ids, weight)
     if weight.dim() != 2 or weight.dtype not in _DTYPES or not 0 < weight.shape[0] <= 1 << 30 or weight.shape[1] == 0:
         raise ValueError(f"embedding: a weight of shape {tuple(weight.shape)} and type {weight.dtype} (2-D float32, bfloat16 or float16)")

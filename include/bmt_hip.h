@@ -662,10 +662,10 @@ int bmt_preference_loss(const void* logits, int dtype, int64_t sb, int64_t st, i
 /* out[n][0 .. D) = scale * W[ids[n]][0 .. D) (W rows at stride ldw, out contiguous, both `dtype`); ids outside [0, V) are clamped as in
  * bmt_prep_embed */
 int bmt_embedding(const int64_t* ids, const void* W, int64_t ldw, void* out, int64_t N, int D, int V, int dtype, float scale, void* stream);
-/* its gradient, the same bits on every run: row v = scale * sum of dout[n] over the positions n with ids[n] == v, added in fp32 in ascending
- * order of n; positions that hold pad_idx, or are clamped to it, are left out (INT64_MIN: none).  dW ([V][D] at stride ldw, `dtype`): every
- * row is written, zeros where a token does not occur -- or into (fp32): the rows of the tokens that occur are added to it.  ws:
- * bmt_embedding_bwd_ws_bytes, 16-byte aligned */
+/* its gradient, the same bits on every run: row v = scale * sum of dout[n] over the positions n with ids[n] == v, added in ascending order of n
+ * (in fp32; a frequent token's sums of up to 32 rows each in 64 bits); positions that hold pad_idx, or are clamped to it, are left out (INT64_MIN:
+ * none).  dW ([V][D] at stride ldw, `dtype`): every row is written, zeros where a token does not occur -- or into (fp32): the rows of the tokens
+ * that occur are added to it, by one atomic addition per element.  ws: bmt_embedding_bwd_ws_bytes, 16-byte aligned */
 int64_t bmt_embedding_bwd_ws_bytes(int64_t N, int D, int V);
 int bmt_embedding_bwd(const int64_t* ids, const void* dout, int64_t ld, int64_t N, int D, int V, int dtype, float scale, int64_t pad_idx, void* dW,
                       float* into, int64_t ldw, void* ws, int64_t ws_bytes, void* stream);

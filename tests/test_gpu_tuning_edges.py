@@ -277,3 +277,29 @@ def test_another_clipping_bound_in_front_of_a_capture_without_warm_up(ops):
     for bound in (-1.0, float("nan")):
         with pytest.raises(ValueError):
             step._clipper.max_norm = bound
+
+
+# ----------------------------------------------------------------------------- embedding
+@pytest.mark.parametrize("static", [False, True])
+@pytest.mark.parametrize("n", [4097, 1 << 22])
+def test_gradient_of_very_frequent_tokens(ops, n, static):
+    """an element's value passes through at most 7 additions of a wave, the 3 that join its four waves, 64 bits from there and one rounding (and one
+    more where it is added to a buffer): 12 u of the absolute sum, however frequent the token is"""
+    V, D, g = 5, 16, gen(n)
+    ids = torch.tensor([0, 3, 4], device="cuda")[torch.randint(0, 3, (n,), device="cuda", generator=g)]
+    ids[7] = 2
+    dout = torch.rand(n, D, device="cuda", generator=g)
+    W = torch.nn.Parameter(torch.randn(V, D, device="cuda", generator=g))
+    want = torch.stack([dout[ids == v].double().sum(0) * 1.5 for v in range(V)])
+    if static:
+        from bmt_amd.parallel import GradientReducer
+        reducer = GradientReducer([W])
+        try:
+            ops.embedding(ids, W, 1.5).backward(dout)
+            got = W.grad.clone()
+        finally:
+            reducer.remove()
+    else:
+        (got,) = torch.autograd.grad(ops.embedding(ids, W, 1.5), W, dout)
+        assert torch.equal(got, torch.autograd.grad(ops.embedding(ids, W, 1.5), W, dout)[0])
+    within(got, want, 12 * U * want, "dW")
