@@ -27,6 +27,13 @@ def within(got, want, tol, name):
     assert not bool(bad.any()), report(got, want, name) + f"\n  {int(bad.sum())} of {bad.numel()} outside"
 
 
+def softmax64(x):
+    """(torch.softmax of float64 rows of more than 1024 elements takes fp32 exponentials on this GPU: up to 1.8e-6 off)"""
+    x = x.detach().double()
+    e = torch.exp(x - x.amax(-1, keepdim=True))
+    return e / e.sum(-1, keepdim=True)
+
+
 # ----------------------------------------------------------------------------- policy loss
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [40, 140001])          # (a row in registers, a row that is read twice)
@@ -46,7 +53,7 @@ def test_gradient_of_the_kl_term_for_any_reference(ops, dtype, V):
     d = ref.double() - lp
     w = -adv.double()[:, None] * torch.exp(lp - old.double()) - beta * torch.expm1(d)
     assert bool(torch.isfinite(w).all())
-    p = torch.softmax(x.detach().double(), -1)
+    p = softmax64(x)
     want = w[..., None] * (torch.zeros_like(p).scatter_(-1, ids[..., None], 1.0) - p)
     # logp is off by less than (3 * 16 + 2) u (one exponential, t = x - max below 16) and a few more of the sum: 64 u; w moves by (|A| + beta e^d) times
     # that and is rounded; p and its product with w: 64 u of |w|; a type of fewer bits adds half a step
@@ -303,3 +310,51 @@ def test_gradient_of_very_frequent_tokens(ops, n, static):
         (got,) = torch.autograd.grad(ops.embedding(ids, W, 1.5), W, dout)
         assert torch.equal(got, torch.autograd.grad(ops.embedding(ids, W, 1.5), W, dout)[0])
     within(got, want, 12 * U * want, "dW")
+
+
+# ----------------------------------------------------------------------------- every element of a gradient, relative to itself
+def test_exponentials_of_an_fp32_gradient_have_no_bias(ops):
+    """exp(t) in a gradient errs by roundings, which average out, and not with t: the mean relative errors of elements near t = -60 and near t = -3
+    differ by less than 2 u.  (The roundings of t log2 e are at most 2.6e-6 there; the mean over 50 000 of them is off by less than six of its own
+    deviations, 6 * 2.6e-6 / 3^1/2 / 50000^1/2 = 4e-8, and 2 u = 1.2e-7.)"""
+    n, g = 50000, gen(5)
+    far, near = -62.0 + 4.0 * torch.rand(n, device="cuda", generator=g), -4.0 + 2.0 * torch.rand(n, device="cuda", generator=g)
+    x = torch.cat([torch.zeros(1, device="cuda"), far, near])[None, None].requires_grad_(True)
+    ids = torch.zeros(1, 1, dtype=torch.int64, device="cuda")
+    want = -softmax64(x)[0, 0, 1:]
+    for loss in (ops.token_logp(x, ids).sum(), ops.policy_loss(x, ids, None, -torch.ones(1, device="cuda"))[0]):
+        (dx,) = torch.autograd.grad(loss, x)
+        rel = (dx[0, 0, 1:].double() / want - 1.0).view(2, n).mean(1)
+        assert abs(float(rel[0] - rel[1])) < 2 * U, rel
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,T,V", [(3, 2, 7), (2, 3, 1000), (5, 7, 4099), (2, 2, 33001), (4, 1, 131075), (2, 1, 300001), (700, 1, 4101), (600, 1, 16385)])
+def test_every_element_of_a_gradient(ops, dtype, B, T, V):
+    """Off the target the gradient is -w p, one product after another, so its error is bounded relative to itself: exp by its argument (t = x - max and
+    t log2 e rounded: 2 |t| u) and the instruction (2 u), 1 / sum (the sum's terms err by (2 |t| + 2) u each, under p |t| averages below ln V + 1 < 14:
+    30 u, and its rounding), two products: (2 |t| + 36) u; the type adds half a step, fp16 half of its smallest one.  At the target w - w p: that of p,
+    and 2 u |w|.  w is exact but for the preference loss, where it is a sigmoid of rewards: beta = 0.1 times 64 u, and its rounding: 8 u more"""
+    g = gen(V + B)
+    x = (torch.randn(B, T, V, device="cuda", generator=g) * 2.5).to(dtype).requires_grad_(True)
+    ids = torch.randint(0, V, (B, T), device="cuda", generator=g)
+    up = torch.randn(B, T, device="cuda", generator=g)
+    x64 = x.detach().double()
+    t = (x64 - x64.amax(-1, keepdim=True)).abs()
+    p = softmax64(x)
+    at = torch.zeros_like(p).scatter_(-1, ids[..., None], 1.0)
+    cases = [("logp", up.double(), 0.0, lambda: (ops.token_logp(x, ids) * up).sum()),
+             ("policy", -up.double(), 0.0, lambda: ops.policy_loss(x, ids, None, up, reduction="sum")[0])]
+    cases.append(("policy times 0.5", -0.5 * up.double(), 0.0, lambda: ops.policy_loss(x, ids, None, up, reduction="sum")[0] * 0.5))
+    if B % 2 == 0 and T == 1:
+        S = torch.log_softmax(x64, -1).gather(-1, ids[..., None])[..., 0].sum(1)
+        z = 0.1 * (S[:B // 2] - S[B // 2:])
+        d = -0.1 / (B // 2) * torch.sigmoid(-z)
+        cases.append(("preference", torch.cat([d, -d])[:, None], 8.0, lambda: ops.preference_loss(x, ids, torch.zeros(B, device="cuda"))[0]))
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for name, w, more, loss in cases:
+        (dx,) = torch.autograd.grad(loss(), x)
+        w = w[..., None]
+        want = w * (at - p)
+        tol = (2 * t + 36 + more) * U * (w * p).abs() + at * (2 + more) * U * w.abs() + HALF[dtype] * want.abs() * (1 + 2.0 ** -8) + tiny
+        within(dx, want, tol, name)
