@@ -134,7 +134,8 @@ class GradientReducer:
         for bi, b in enumerate(self.buckets):
             for si, p in enumerate(b["params"]):
                 self._slot[p] = (bi, si)
-        self._hooks = [p.register_post_accumulate_grad_hook(self._on_grad) for p in params]
+        self._accumulated, self._final = set(), set()      # ids of parameters: autograd's own node has run / the gradient is final, in this pass
+        self._hooks = [p.register_post_accumulate_grad_hook(self._on_accumulated) for p in params]
         for p in params:       # lets the fused weight-gradient path (ops.static_grad / ops.grad_done) find its buffer and report
             p._bmt_static_grad = True
             p._bmt_on_grad = self._on_grad
@@ -199,20 +200,37 @@ class GradientReducer:
                 if p.grad is not v:
                     p.grad = v
                 p._bmt_uses = 0
+        self._accumulated.clear()
+        self._final.clear()
         self._handles = []
         self._second = []
         if self._arena is not None and self._arena.is_cuda:      # a new step: nothing of the last one is left to settle
             from . import ops as _ops
             _ops.context().gen_handles.clear()
 
-    def _on_grad(self, p):
+    # A parameter's gradient is final once autograd's own node for it has run -- its hook is called whether a tensor arrived or the nodes in front of
+    # it added theirs to the buffer and returned none -- AND the last of those additions is on the stream (ops.grad_done: a queued product may come
+    # long behind the hook).  Either alone would let a bucket be summed over the ranks too early, and both together twice.
+    def _on_accumulated(self, p):
         bi, si = self._slot[p]
-        b = self.buckets[bi]
-        v = b["views"][si]
+        v = self.buckets[bi]["views"][si]
         if p.grad.data_ptr() != v.data_ptr():
             # autograd replaced the tensor (grad was None): copy into the bucket and re-bind
             v.copy_(p.grad)
             p.grad = v
+        self._accumulated.add(id(p))
+        if getattr(p, "_bmt_uses", 0) <= 0:
+            self._settle(p)
+
+    def _on_grad(self, p):
+        if id(p) in self._accumulated:
+            self._settle(p)
+
+    def _settle(self, p):
+        if id(p) in self._final:
+            return
+        self._final.add(id(p))
+        b = self.buckets[self._slot[p][0]]
         b["pending"] -= 1
         if b["pending"] == 0 and self.world > 1 and self.overlap:
             self._reduce_bucket(b)

@@ -358,3 +358,45 @@ def test_every_element_of_a_gradient(ops, dtype, B, T, V):
         want = w * (at - p)
         tol = (2 * t + 36 + more) * U * (w * p).abs() + at * (2 + more) * U * w.abs() + HALF[dtype] * want.abs() * (1 + 2.0 ** -8) + tiny
         within(dx, want, tol, name)
+
+
+# ----------------------------------------------------------------------------- gradient buckets
+@pytest.mark.parametrize("name", LOSSES)
+def test_buckets_behind_a_loss_on_a_generator_s_output(ops, name):
+    """every bucket is handed to its collective once, with the gradients that the pass ends with"""
+    from bmt_amd.parallel import GradientReducer
+    generator, x, losses = behind_a_generator()
+    reducer = GradientReducer([generator.linear.weight, generator.linear.bias], bucket_bytes=1)
+    reducer.world, handed = 2, []          # (as one of two ranks; the collective is this list)
+    reducer._reduce_bucket = lambda b: handed.append((b["flat"], b["flat"].clone()))
+    try:
+        for _ in range(2):
+            handed.clear()
+            reducer.zero_grad()
+            losses[name](generator(x)).backward()
+            assert len(handed) == len(reducer.buckets) == 2
+            reducer.finish()
+            assert len(handed) == 2 and all(torch.equal(flat, at) and bool((at != 0).any()) for flat, at in handed)
+    finally:
+        reducer.remove()
+
+
+def test_buckets_of_an_overlapped_step_are_reduced_once_and_complete(ops):
+    from tests.test_gpu_tuning import caption_step
+    single, fs, caps = caption_step(None)
+    from bmt_amd.train import CaptioningTrainStep
+    step = CaptioningTrainStep(single.model, single.cfg, single.pad_idx, data_parallel=True, bucket_bytes=1 << 14)
+    reducer, handed = step.reducer, []
+    reducer.world = 2
+    reducer._reduce_bucket = lambda b: handed.append((b["flat"], b["flat"].clone()))
+    assert len(reducer.buckets) > 4
+    for _ in range(2):
+        handed.clear()
+        kl, n = step._forward_backward(fs, caps)
+        inside = len(handed)
+        step._reduce(kl, n)
+        assert inside > 0 and len(handed) == len(reducer.buckets)
+        assert sorted(f.data_ptr() for f, _ in handed) == sorted(b["flat"].data_ptr() for b in reducer.buckets)
+        assert all(torch.equal(flat, at) for flat, at in handed)
+        step._optimize()
+    reducer.remove()
