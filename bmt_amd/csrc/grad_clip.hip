@@ -3,14 +3,14 @@
 // over any number of fp32 / bf16 / fp16 tensors (s: an optional scale of all gradients that the caller has not applied yet).
 // Bound: HBM -- the norm reads every gradient once, and nothing can be written before it is known, so clipping reads them a second time.
 // Two launches: `norm` leaves one 64-bit partial sum per workgroup; every workgroup of `apply` adds those (they come from L2), in one order, and
-// scales its tiles, walking them backwards: the tiles the norm read last are the ones the memory-side cache still holds.  The norm's loads are
-// ordinary ones for that reason; those and the stores of `apply` pass the caches by (nontemporal: 120 -> 97 us for 50 M fp32 values, 488 -> 424 us
-// for 313 M bf16 values into fp32; with nontemporal loads in the norm, too, 104 and 433 us).
-// Squares and sums are 64-bit: a product of two fp32 values is exact there and cannot leave the range, and HBM leaves the time for it (fp32 squares:
-// 97.6 and 425 us, the same).  No atomics.
+// scales its tiles, in the order in which `norm` read them (backwards, for what a cache might still hold of the last ones: 97 us for 93 at 50 M fp32
+// values, 194 for 186 at 100 M, 424 for 414 at 313 M bf16 values into fp32).  The norm's loads are ordinary ones, the loads and stores of `apply` pass
+// the caches by: with ordinary loads there 98, 216 and 466 us, with nontemporal ones in the norm, too, 104 and 433 (50 M, 313 M; against 97 and 424).
+// Squares and sums are 64-bit: a product of two fp32 values is exact there and cannot leave the range, and HBM leaves the time for it (fp32 squares took
+// the same).  No atomics.
 // The tensors are cut into tiles (of 32 KB: 8 loads of 16 bytes in flight per thread) by the caller's table, so a model of 200 tensors and one arena
-// load the chip alike.  Measured: 50 M fp32 values 34 us for the norm (5.9 TB/s) and 63 us for reading again and writing (6.4 TB/s); 313 M bf16 values into
-// fp32 104 us (6.0 TB/s) and 320 us (5.9 TB/s).
+// load the chip alike.  Measured: 50 M fp32 values 33 us for the norm (6.0 TB/s) and 61 us for reading again and writing (6.6 TB/s); 313 M bf16 values into
+// fp32 105 us (6.0 TB/s) and 311 us (6.0 TB/s).
 #include "common.h"
 
 namespace {
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256) void clip_apply_kernel(const Tile* __restrict_
         result[1] = c;
     }
     if (in_place && c == 1.f) return;
-    for (int i = n - 1 - (int)blockIdx.x; i >= 0; i -= (int)gridDim.x) {
+    for (int i = (int)blockIdx.x; i < n; i += (int)gridDim.x) {
         const Tile t = tiles[i];
         const int dt = t.kind & 3;
         if (dt == BMT_DT_F32) scale_to<BMT_DT_F32>(t, c);

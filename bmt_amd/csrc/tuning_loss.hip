@@ -10,8 +10,8 @@
 // sequence in 64 bits; 16-bit gradients are rounded once.  No atomics: results do not depend on the schedule.
 // Rows that do not count (mask 0, or the padding id) are not read; their gradient rows are written as zeros.
 // Measured: policy loss with its gradient, all rows counting, 8192 x 32000 bf16 202 us (5.2 TB/s of logits read + gradients written; a plain copy
-// reaches 5.95), 65536 x 1000 bf16 78 us; preference loss 16 x 1024 x 32000 bf16, a third of the rows masked: 121 us for the log-probabilities (5.7 TB/s
-// of the rows read), 291 us for the gradient (5.9 TB/s).
+// reaches 5.95), 65536 x 1000 bf16 78 us; preference loss 16 x 1024 x 32000 bf16, a third of the rows masked: 123 us for the log-probabilities (5.4 TB/s
+// of the rows read), 280 us for the gradient (6.1 TB/s).
 #include "common.h"
 
 namespace {
@@ -187,8 +187,9 @@ struct Row {
     }
     __device__ __forceinline__ int granules() const { return (end + E::G - 1) / E::G; }
     __device__ __forceinline__ bool inner(int k) const { return k * E::G >= phase && (k + 1) * E::G <= end; }
-    // LAST: nothing reads the row again, and the load passes the caches by, as the gradient's stores do (16 x 1024 x 32000 bf16 preference pass: 460 us
-    // without any of it, 441 with all loads like that, 416 with the forward pass's left to the caches, whose end the gradient kernel reads first)
+    // LAST: nothing reads the row again, and the load passes the caches by, as the gradient's stores do.  A preference pass over all rows of 16 x 1024 x
+    // 32000 bf16 takes 557 us; 595 with ordinary loads in the gradient kernel, 614 with ordinary stores there, 568 with the forward pass's loads past the
+    // caches, too; 16 x 128 x 32000 fp32, of which the memory-side cache keeps much: 141, 142, 183, 169
     template <bool LAST>
     __device__ __forceinline__ u32x4 load(int k) const {
         const char* p = base + (int64_t)k * 16;
@@ -589,8 +590,7 @@ __global__ __launch_bounds__(NT) void logit_grad_kernel(Rows q, const float2* __
     using E = Elem<DT>;
     const float gs = g ? g[0] : 1.f;
     if (once && gs == 1.f) return;
-    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-        const int64_t r = rows - 1 - i;      // last rows first: what the forward pass read last is what the memory-side cache still holds
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const int b = (int)((unsigned)r / (unsigned)q.T), t = (int)((unsigned)r % (unsigned)q.T);
         const int64_t id = q.id[b * q.ib + t * q.it];
         const char* xr = q.x + (b * q.sb + t * q.st) * E::B;
