@@ -11,8 +11,8 @@
 //   sum    a wave per (token, block of columns) adds a token's rows if they are at most EMB_LONG; the rows of more frequent tokens are added
 //          EMB_LONG sorted positions at a time by workgroups of their own (a few tokens hold half of a text)
 //   join   adds those partial sums per token, in order
-// Measured (bf16, 65536 Zipf-distributed ids, 32000 x 1024 table): lookup 29 us (6.9 TB/s of distinct rows read + rows written); gradient 67 us for
-// 200 MB: order 17 us in three launches, sum 37 us (5.4 TB/s), join 5 us.  An odd width (1021) costs the same within 2 us (93 and 129 us when such
+// Measured (bf16, 65536 Zipf-distributed ids, 32000 x 1024 table): lookup 36 us in a pass with its gradient (5.6 TB/s of distinct rows read + rows
+// written; 29 us alone, again and again); gradient 60 us for 200 MB: order 17 us in three launches, sum 37 us (5.4 TB/s), join 5 us.  An odd width (1021) costs the same within 2 us (93 and 129 us when such
 // rows were read element by element).
 #include "common.h"
 

@@ -24,7 +24,7 @@ constexpr int DA = 128, TS = 68;
 
 typedef float v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void tile_mac(const float* As, const float* Bs, int ty, int tx, float (&acc)[4][4]) {
-    v2f c[4][2];                     // packed multiply-adds (v_pk_fma_f32): two columns per instruction
+    v2f c[4][2];                     // two columns side by side
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         c[i][0] = v2f{acc[i][0], acc[i][1]};
