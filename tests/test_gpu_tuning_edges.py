@@ -400,3 +400,31 @@ def test_buckets_of_an_overlapped_step_are_reduced_once_and_complete(ops):
         assert all(torch.equal(flat, at) for flat, at in handed)
         step._optimize()
     reducer.remove()
+
+
+def test_buckets_of_an_overlapped_proposal_step_are_reduced_once_and_complete(ops, golden):
+    """the same where products run as autograd reaches them, weights are read through views, and the reduction ends inside the step"""
+    from bmt_amd.model.proposal_generator import MultimodalProposalGenerator
+    from bmt_amd.train import ProposalTrainStep
+    from tests.test_gpu_proposal import _prop_cfg
+    g, cfg = golden("tiny_prop.npz"), _prop_cfg()
+    cfg.lr, cfg.grad_clip = 1e-3, None
+    model = MultimodalProposalGenerator(cfg, {"audio": [float(a) for a in g.np("anchors_audio")], "video": [float(a) for a in g.np("anchors_video")]})
+    model.load_state_dict(g.sub("sd/"))
+    step = ProposalTrainStep(model.cuda(), cfg, pad_idx=1, data_parallel=True, bucket_bytes=1 << 12)
+    reducer, handed, checks = step.reducer, [], []
+    reducer.world = 2
+    reducer._reduce_bucket = lambda b: handed.append((b["flat"], b["flat"].clone()))
+
+    def finish(inner=reducer.finish):
+        inside = len(handed)
+        inner()
+        checks.append((inside, len(handed), all(torch.equal(flat, at) for flat, at in handed)))
+    reducer.finish = finish
+    fs, targets = {k: g[k].cuda() for k in ("rgb", "flow", "audio")}, g["targets"].cuda()
+    for _ in range(2):
+        handed.clear()
+        step(fs, targets)
+    n = len(reducer.buckets)
+    assert n > 4 and checks == [(n, n, True)] * 2
+    reducer.remove()
